@@ -60,6 +60,13 @@ EXPORTED = (
     "fgw_mha_static_ws_read_error",
     "fgw_mha_selftest_wait",
     "fgw_paged_cache_gather",
+    "fgw_rotary_append",
+    "fgw_chunk_workspace_size",
+    "fgw_chunk_attention",
+    "fgw_page_workspace_size",
+    "fgw_page_fork",
+    "fgw_page_compact",
+    "fgw_page_copy",
 )
 
 STATIC_WORKSPACE_BYTES = 16 << 20  # FGW_MHA_STATIC_WORKSPACE_BYTES
@@ -167,6 +174,42 @@ class GatherParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``fgw_rotary_params`` (include/fgw_mha.h)."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("q", "k", "v", "q_out", "k_cache", "v_cache", "block_table",
+                                                     "cache_seqlens", "cu_seqlens_q", "cos_sin")]
+    _fields_ += [(name, ctypes.c_int64) for name in ("tokens", "pool_rows", "q_stride", "k_stride", "v_stride",
+                                                     "q_out_stride")]
+    _fields_ += [(name, ctypes.c_int32) for name in ("batch", "heads", "kv_heads", "head_dim", "rotary_dim",
+                                                     "positions", "table_width", "page_size", "dtype", "interleaved")]
+    _fields_ += [("reserved", ctypes.c_int32 * 2)]
+
+
+class ChunkParams(ctypes.Structure):
+    """Mirror of ``fgw_chunk_params`` (include/fgw_mha.h)."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("q", "k_cache", "v_cache", "block_table", "cache_seqlens",
+                                                     "cu_seqlens_q", "out")]
+    _fields_ += [(name, ctypes.c_int64) for name in ("tokens", "pool_rows", "q_stride", "out_stride")]
+    _fields_ += [(name, ctypes.c_int32) for name in ("batch", "heads", "kv_heads", "head_dim", "table_width",
+                                                     "page_size", "dtype", "causal")]
+    _fields_ += [("softmax_scale", ctypes.c_float), ("wait_budget_ms", ctypes.c_int32),
+                 ("reserved", ctypes.c_int32 * 2)]
+
+
+class PageParams(ctypes.Structure):
+    """Mirror of ``fgw_page_params`` (include/fgw_mha.h)."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("pools", "block_table", "cache_seqlens", "parents",
+                                                     "reserve_seqlens", "table_out", "seqlens_out", "status",
+                                                     "src_pages", "dst_pages")]
+    _fields_ += [("row_bytes", ctypes.c_int64)]
+    _fields_ += [(name, ctypes.c_int32) for name in ("pool_count", "batch", "table_width", "page_size", "num_pages",
+                                                     "copy_count")]
+    _fields_ += [("reserved", ctypes.c_int32 * 2)]
+
+
 _LIB = None
 
 
@@ -221,6 +264,16 @@ def library():
     lib.fgw_mha_static_ws_read_error.restype = ctypes.c_int
     lib.fgw_paged_cache_gather.argtypes = [ctypes.POINTER(GatherParams), vp]
     lib.fgw_paged_cache_gather.restype = ctypes.c_int
+    lib.fgw_rotary_append.argtypes = [vp, vp]
+    lib.fgw_rotary_append.restype = ctypes.c_int
+    for name in ("fgw_chunk_workspace_size", "fgw_page_workspace_size"):
+        fn = getattr(lib, name)
+        fn.argtypes = [vp, ctypes.POINTER(ctypes.c_size_t)]
+        fn.restype = ctypes.c_int
+    for name in ("fgw_chunk_attention", "fgw_page_fork", "fgw_page_compact", "fgw_page_copy"):
+        fn = getattr(lib, name)
+        fn.argtypes = [vp, vp, ctypes.c_size_t, vp]
+        fn.restype = ctypes.c_int
     _LIB = lib
     return lib
 
@@ -338,3 +391,39 @@ def paged_cache_gather(params, stream_ptr):
     """``fgw_paged_cache_gather``: pack the cache rows the requests reach into ``params.dst``."""
     check(library().fgw_paged_cache_gather(ctypes.byref(params), ctypes.c_void_p(stream_ptr)),
           "fgw_paged_cache_gather")
+
+
+def rotary_append(params, stream_ptr):
+    """``fgw_rotary_append``: rotate the new tokens' queries and keys and append keys and values to the cache."""
+    check(library().fgw_rotary_append(ctypes.byref(params), stream_ptr), "fgw_rotary_append")
+
+
+def chunk_workspace_size(params):
+    out = ctypes.c_size_t(0)
+    check(library().fgw_chunk_workspace_size(ctypes.byref(params), ctypes.byref(out)), "fgw_chunk_workspace_size")
+    return out.value
+
+
+def chunk_attention(params, workspace_ptr, workspace_bytes, stream_ptr):
+    """``fgw_chunk_attention``: attention of the new tokens over the cache."""
+    check(library().fgw_chunk_attention(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr),
+          "fgw_chunk_attention")
+
+
+def page_workspace_size(params):
+    out = ctypes.c_size_t(0)
+    check(library().fgw_page_workspace_size(ctypes.byref(params), ctypes.byref(out)), "fgw_page_workspace_size")
+    return out.value
+
+
+def page_fork(params, workspace_ptr, workspace_bytes, stream_ptr):
+    check(library().fgw_page_fork(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_fork")
+
+
+def page_compact(params, workspace_ptr, workspace_bytes, stream_ptr):
+    check(library().fgw_page_compact(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr),
+          "fgw_page_compact")
+
+
+def page_copy(params, workspace_ptr, workspace_bytes, stream_ptr):
+    check(library().fgw_page_copy(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_copy")

@@ -465,6 +465,83 @@ int fgw_paged_cache_gather(const fgw_gather_params* params, void* stream) {
   return launch_gather(*params, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FGW_OK : FGW_ERR_CUDA;
 }
 
+// The current device and its SM count for a call that has passed its argument checks.
+static int current_device(int* device, int* sms) {
+  if (cudaGetDevice(device) != cudaSuccess) return FGW_ERR_NO_DEVICE;
+  return device_sm_count_cached(*device, sms);
+}
+
+int fgw_rotary_append(const fgw_rotary_params* params, void* stream) {
+  if (params == nullptr) return FGW_ERR_INVALID_ARGUMENT;
+  int st = rotary_validate(*params);
+  if (st != FGW_OK || params->tokens == 0) return st;
+  int device = 0, sms = 0;
+  st = current_device(&device, &sms);
+  if (st != FGW_OK) return st;
+  return launch_rotary(*params, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FGW_OK : FGW_ERR_CUDA;
+}
+
+int fgw_chunk_workspace_size(const fgw_chunk_params* params, size_t* bytes) {
+  if (params == nullptr || bytes == nullptr) return FGW_ERR_INVALID_ARGUMENT;
+  const int st = chunk_validate(*params);
+  if (st == FGW_OK) *bytes = chunk_workspace_bytes(*params);
+  return st;
+}
+
+int fgw_chunk_attention(const fgw_chunk_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  if (params == nullptr) return FGW_ERR_INVALID_ARGUMENT;
+  int st = chunk_validate(*params);
+  if (st != FGW_OK || params->tokens == 0) return st;
+  st = chunk_validate_pointers(*params);
+  if (st != FGW_OK) return st;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return FGW_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < chunk_workspace_bytes(*params)) return FGW_ERR_WORKSPACE_TOO_SMALL;
+  int device = 0, sms = 0;
+  st = current_device(&device, &sms);
+  if (st != FGW_OK) return st;
+  const cudaError_t err = launch_chunk(*params, workspace, sms, device, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? FGW_OK : FGW_ERR_CUDA;
+}
+
+static int page_workspace_size(const fgw_page_params* params, int op, size_t* bytes) {
+  if (params == nullptr || bytes == nullptr) return FGW_ERR_INVALID_ARGUMENT;
+  if (params->batch < 0 || params->num_pages <= 0 || params->num_pages > (1 << 30) || params->copy_count < 0) {
+    return FGW_ERR_INVALID_ARGUMENT;
+  }
+  *bytes = page_workspace_bytes(*params, op);
+  return FGW_OK;
+}
+
+static int page_op(const fgw_page_params* params, int op, void* workspace, size_t workspace_bytes, void* stream) {
+  if (params == nullptr) return FGW_ERR_INVALID_ARGUMENT;
+  int st = page_validate(*params, op);
+  if (st != FGW_OK) return st;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return FGW_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < page_workspace_bytes(*params, op)) return FGW_ERR_WORKSPACE_TOO_SMALL;
+  int device = 0, sms = 0;
+  st = current_device(&device, &sms);
+  if (st != FGW_OK) return st;
+  const cudaError_t err = launch_page_op(*params, op, workspace, sms, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? FGW_OK : FGW_ERR_CUDA;
+}
+
+int fgw_page_workspace_size(const fgw_page_params* params, size_t* bytes) {
+  if (params != nullptr && params->batch == 0) return page_workspace_size(params, kPageCopy, bytes);
+  return page_workspace_size(params, kPageFork, bytes);
+}
+
+int fgw_page_fork(const fgw_page_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  return page_op(params, kPageFork, workspace, workspace_bytes, stream);
+}
+
+int fgw_page_compact(const fgw_page_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  return page_op(params, kPageCompact, workspace, workspace_bytes, stream);
+}
+
+int fgw_page_copy(const fgw_page_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  return page_op(params, kPageCopy, workspace, workspace_bytes, stream);
+}
+
 int fgw_mha_read_error(const void* workspace, void* stream, int* device_status, int* site) {
   if (workspace == nullptr || device_status == nullptr) return FGW_ERR_INVALID_ARGUMENT;
   if (cudaStreamSynchronize(static_cast<cudaStream_t>(stream)) != cudaSuccess) return FGW_ERR_CUDA;

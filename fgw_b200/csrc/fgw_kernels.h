@@ -100,6 +100,20 @@ void carve_workspace(LaunchDesc& d, void* workspace, int path);
 // Paged-cache gather (fgw_gather.cu): argument check (an fgw_status) and launch.
 int gather_validate(const fgw_gather_params& p);
 cudaError_t launch_gather(const fgw_gather_params& p, int sm_count, cudaStream_t stream);
+// Rotary positions and cache append (fgw_rotary.cu).
+int rotary_validate(const fgw_rotary_params& p);
+cudaError_t launch_rotary(const fgw_rotary_params& p, int sm_count, cudaStream_t stream);
+// Attention of new tokens over the cache (fgw_chunk.cu): argument checks (an fgw_status) and launch.
+constexpr int kMaxGroup = 128;  // query heads that may share a key head
+int chunk_validate(const fgw_chunk_params& p);
+int chunk_validate_pointers(const fgw_chunk_params& p);
+size_t chunk_workspace_bytes(const fgw_chunk_params& p);
+cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_count, int device, cudaStream_t stream);
+// Page-table operators (fgw_pages.cu).
+enum PageOp { kPageFork = 0, kPageCompact = 1, kPageCopy = 2 };
+int page_validate(const fgw_page_params& p, int op);
+size_t page_workspace_bytes(const fgw_page_params& p, int op);
+cudaError_t launch_page_op(const fgw_page_params& p, int op, void* workspace, int sm_count, cudaStream_t stream);
 cudaError_t launch_plan(const LaunchDesc& d);
 // fused_merge (with write_partials): the CTA completing a group's split set merges it into the output.
 cudaError_t launch_decode(const LaunchDesc& d, bool write_partials, bool fused_merge);

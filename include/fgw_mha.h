@@ -286,6 +286,134 @@ typedef struct fgw_gather_params {
 
 FGW_API int fgw_paged_cache_gather(const fgw_gather_params* params, void* stream);
 
+/*
+ * Operators of a serving step around the attention (no reference counterpart: FGW's callers bring rotated keys in a filled
+ * cache, one query length per batch and as many key heads as query heads).
+ *
+ * Ragged batches: request b's new tokens are rows cu_seqlens_q[b] <= t < cu_seqlens_q[b + 1] of q, k, v and out, in
+ * order; cache_seqlens[b] counts its tokens in the cache WITH the new ones, so the i-th of n new tokens has position
+ * cache_seqlens[b] - n + i. All lengths stay device data: no call copies to the host or synchronises. cu_seqlens_q is
+ * non-decreasing; lengths are clamped into [0, table_width * page_size].
+ */
+
+/*
+ * Rotary positions and cache append. The first rotary_dim values of every query and key head turn by the angles of the
+ * token's position, cos_sin[position] = rotary_dim / 2 cosines, then as many sines: pair (x, y) becomes
+ * (x cos - y sin, y cos + x sin) in FP32, rounded once; pairs are values (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when
+ * interleaved; the other values pass unchanged. Rotated queries go to q_out (q itself is allowed), rotated keys and
+ * the values to the cache row of the position. Rows of no request, and positions below 0, past the page table or
+ * past cos_sin, give zeros in q_out and append nothing; a page id outside the pool appends nothing.
+ */
+typedef struct fgw_rotary_params {
+  const void* q;               /* [tokens, heads, head_dim], q_stride elements from token to token */
+  const void* k;               /* [tokens, kv_heads, head_dim], k_stride */
+  const void* v;               /* [tokens, kv_heads, head_dim], v_stride */
+  void* q_out;                 /* [tokens, heads, head_dim], q_out_stride, written */
+  void* k_cache;               /* [pool_rows, kv_heads, head_dim] contiguous, written */
+  void* v_cache;               /* [pool_rows, kv_heads, head_dim] contiguous, written */
+  const int32_t* block_table;  /* [batch, table_width] */
+  const int32_t* cache_seqlens; /* [batch] */
+  const int32_t* cu_seqlens_q; /* [batch + 1] */
+  const float* cos_sin;        /* [positions, rotary_dim] */
+  int64_t tokens;
+  int64_t pool_rows;           /* a multiple of page_size */
+  int64_t q_stride, k_stride, v_stride, q_out_stride; /* multiples of 8 elements; bases 16-byte aligned */
+  int32_t batch;
+  int32_t heads;               /* a multiple of kv_heads */
+  int32_t kv_heads;
+  int32_t head_dim;            /* 16..256, multiple of 16 */
+  int32_t rotary_dim;          /* even, 2..head_dim */
+  int32_t positions;           /* rows of cos_sin */
+  int32_t table_width;
+  int32_t page_size;
+  int32_t dtype;               /* FGW_DTYPE_FLOAT16 or FGW_DTYPE_BFLOAT16 */
+  int32_t interleaved;         /* 0 or 1 */
+  int32_t reserved[2];         /* must be zero */
+} fgw_rotary_params;
+
+FGW_API int fgw_rotary_append(const fgw_rotary_params* params, void* stream);
+
+/*
+ * Attention of the new tokens over the cache: query head h of a token reads key head h / (heads / kv_heads). Causal: the
+ * i-th of n new tokens sees the first cache_seqlens - n + i + 1 cached tokens; otherwise all of them. Rows that see
+ * nothing, and rows of no request, are written as zeros. Page ids are trusted, as in fgw_mha_paged_fwd. Results are the
+ * same bits from call to call.
+ */
+typedef struct fgw_chunk_params {
+  const void* q;               /* [tokens, heads, head_dim], q_stride elements from token to token */
+  const void* k_cache;         /* [pool_rows, kv_heads, head_dim] contiguous */
+  const void* v_cache;         /* [pool_rows, kv_heads, head_dim] contiguous */
+  const int32_t* block_table;  /* [batch, table_width] */
+  const int32_t* cache_seqlens; /* [batch] */
+  const int32_t* cu_seqlens_q; /* [batch + 1] */
+  void* out;                   /* [tokens, heads, head_dim], out_stride, written */
+  int64_t tokens;
+  int64_t pool_rows;           /* a multiple of page_size */
+  int64_t q_stride, out_stride; /* multiples of 8 elements; bases 16-byte aligned */
+  int32_t batch;
+  int32_t heads;               /* a multiple of kv_heads, at most 128 times it */
+  int32_t kv_heads;
+  int32_t head_dim;            /* 16..256, multiple of 16 */
+  int32_t table_width;
+  int32_t page_size;           /* a multiple of 16 */
+  int32_t dtype;               /* FGW_DTYPE_FLOAT16 or FGW_DTYPE_BFLOAT16 */
+  int32_t causal;              /* 0 or 1 */
+  float softmax_scale;         /* positive */
+  int32_t wait_budget_ms;      /* device-side wait limit; 0 = default (2000 ms) */
+  int32_t reserved[2];         /* must be zero */
+} fgw_chunk_params;
+
+/* Bytes of device workspace fgw_chunk_attention needs (by the shapes alone; pointers may be NULL). */
+FGW_API int fgw_chunk_workspace_size(const fgw_chunk_params* params, size_t* bytes);
+
+/* `workspace` must be 256-byte aligned device memory; fgw_mha_read_error reads its device-side status. */
+FGW_API int fgw_chunk_attention(const fgw_chunk_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Page-table operators. Row b of block_table holds the pages of its first cache_seqlens[b] tokens; a page that no row
+ * holds is free. Entries of table_out past a row's pages are -1. Page ids outside [0, num_pages) are passed on and
+ * never read or written. The pools are the K and V caches of every layer, of one shape: pools[i] is
+ * [num_pages * page_size] rows of row_bytes bytes each.
+ */
+typedef struct fgw_page_params {
+  void* const* pools;           /* [pool_count] device pointers, in host memory; 16-byte aligned */
+  const int32_t* block_table;   /* [batch, table_width] */
+  const int32_t* cache_seqlens; /* [batch] */
+  const int32_t* parents;       /* [batch], fork only */
+  const int32_t* reserve_seqlens; /* [batch] or NULL, fork only */
+  int32_t* table_out;           /* [batch, table_width], not block_table */
+  int32_t* seqlens_out;         /* [batch], fork only, not cache_seqlens */
+  int32_t* status;              /* [2], written */
+  const int32_t* src_pages;     /* [copy_count], copy only */
+  const int32_t* dst_pages;     /* [copy_count], copy only */
+  int64_t row_bytes;            /* bytes of one token's row in a pool, a multiple of 16 */
+  int32_t pool_count;           /* 0: tables only */
+  int32_t batch;
+  int32_t table_width;
+  int32_t page_size;
+  int32_t num_pages;            /* at most 2^30 */
+  int32_t copy_count;           /* copy only */
+  int32_t reserved[2];          /* must be zero */
+} fgw_page_params;
+
+/* Bytes of device workspace the page operators need (batch 0: fgw_page_copy's). */
+FGW_API int fgw_page_workspace_size(const fgw_page_params* params, size_t* bytes);
+
+/* Every row i becomes a fork of row parents[i] as it was (its own index keeps it; an index outside [0, batch) frees the
+ * row): the parent's full pages are shared; its partly filled last page stays with the first row that has this parent
+ * and is copied for the others (the filled token rows, in every pool); reserve_seqlens[i] tokens (no fewer than the
+ * parent's) get pages. New pages are the lowest free ones, given in (row, column) order. status = {pages needed, pages
+ * free}; when more are needed than free, the outputs are the inputs and nothing is copied. */
+FGW_API int fgw_page_fork(const fgw_page_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Moves the held pages into the lowest ids: with `live` pages held, the k-th held page from id `live` on goes to the k-th
+ * free page below it, in every pool. status = {live, pages moved}. */
+FGW_API int fgw_page_compact(const fgw_page_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies page src_pages[i] to page dst_pages[i] in every pool. No destination may be a source or occur twice; pairs with a
+ * page outside the pool are skipped. */
+FGW_API int fgw_page_copy(const fgw_page_params* params, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
