@@ -1,0 +1,637 @@
+// Chunk attention, tensor kernel (tcgen05): requests with more than 16 (token, query head) rows per key head.
+//
+// Rows of a 128-row tile are (token, query head of the group) pairs of one key head, token by token: 128 / G tokens of G
+// heads. One TMA box {64 values, G heads, 128 / G tokens} loads such a tile from the queries as they lie in memory, and
+// each K/V tile serves all heads of the group.
+//
+// Up to D = 128 a work item is two tiles (A, B) that share every K/V tile. Per K/V tile j the MMA warp issues PV_A(j),
+// QK_A(j + 1), PV_B(j), QK_B(j + 1), so the softmax of one tile overlaps the other's MMAs; S and O live in TMEM and P
+// overwrites the S columns it came from (TS-form PV). Above 128, O takes 256 columns and an item is one tile.
+// TMEM: S_t at column 128 t, O_A at 256, O_B at 384.
+//
+// Bound by the tensor and special-function units together: a tile pair costs 2048 cycles of MMA at D = 128 and as many of
+// 2^x, and S shares its columns with P, so both must overlap tile against tile.
+#include <algorithm>
+
+#include "fgw_chunk.cuh"
+
+namespace fgw {
+
+template <int NB>
+struct TensorShape {
+  static constexpr int kTiles = chunk_tensor_tiles(NB);
+  static constexpr int kBN = 128;
+  static constexpr int kTileBytes = 128 * 128;         // one 64-value block of a 128-row operand
+  static constexpr int kQBytes = NB * kTileBytes;      // one query tile
+  static constexpr int kKVBytes = NB * kBN * 128;      // one K (or V) stage
+  static constexpr int kStages = NB == 1 ? 4 : (NB == 2 ? 2 : 1);
+  static constexpr int kThreads = 128 + 128 * kTiles;
+  // two-tile kernel: registers per thread after the warpgroup split (4 x 32 x 88 + 8 x 32 x 208 = 384 x 168)
+  static constexpr int kRegsControl = 88;
+  static constexpr int kRegsSoftmax = 208;
+  __device__ __forceinline__ static uint32_t s_col(int t) { return static_cast<uint32_t>(t) * 128u; }
+  __device__ __forceinline__ static uint32_t o_col(int t) { return 256u + static_cast<uint32_t>(t) * 128u; }
+  static constexpr int kTmemCols = 512;
+  static constexpr int kK = kTiles * kQBytes;
+  static constexpr int kV = kK + kStages * kKVBytes;
+  static constexpr int kBar = kV + kStages * kKVBytes;
+  // q_full, q_empty, {k,v}_{full,empty}[S], s_full, p_half, p_full, pv_done, o_empty [2], mma_done
+  static constexpr int kNumBars = 2 + 4 * kStages + 10 + 1;
+  static constexpr int kTmemSlot = kBar + kNumBars * 8;
+  static constexpr int kBytes = kTmemSlot + 16 + 1024;
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
+};
+
+// max(a, b, c) in one instruction (sm_100 three-input max; NaN-free inputs here)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^(s * scale - m) for 64 scores, packed to 16-bit pairs; the row sum adds the rounded values PV multiplies (with the
+// lazily rescaled maximum a row's largest P may exceed 1 and round, and that rounding must cancel).
+template <typename Tr>
+__device__ __forceinline__ void exp2_pack64(const uint32_t* sr, float2 scale2, float2 negm2, float2 (&acc)[4],
+                                            uint32_t (&packed)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), scale2, negm2);
+    packed[i] = Tr::pack2(fast_exp2(x.x), fast_exp2(x.y));
+    acc[i % 4] = Tr::add2(acc[i % 4], packed[i]);
+  }
+}
+
+// Tiles of the segment that query tile t works on, and its first token within the item.
+__device__ __forceinline__ int tile_steps(const ChunkArgs& a, const ChunkSegment& s, int t, int tokens) {
+  const int left = s.count - t * tokens;
+  if (left <= 0) return 0;
+  const int seen = seen_keys(a, s, t * tokens + min(left, tokens) - 1);
+  return max(0, min(s.n_begin + s.n, (seen + 127) / 128) - s.n_begin);
+}
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
+    chunk_tensor_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ ChunkArgs a) {
+  using S = TensorShape<NB>;
+  using Tr = ElemTraits<T>;
+  constexpr int BN = S::kBN, NS = S::kStages, kTiles = S::kTiles;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_smem = smem;
+  uint8_t* k_smem = smem + S::kK;
+  uint8_t* v_smem = smem + S::kV;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;
+  uint64_t* k_empty = k_full + NS;
+  uint64_t* v_full = k_empty + NS;
+  uint64_t* v_empty = v_full + NS;
+  uint64_t* s_full = v_empty + NS;  // [2]
+  uint64_t* p_half = s_full + 2;    // [2]: the first 64 keys of P_t are in TMEM
+  uint64_t* p_full = p_half + 2;    // [2]
+  uint64_t* pv_done = p_full + 2;   // [2]
+  uint64_t* o_empty = pv_done + 2;  // [2]
+  uint64_t* mma_done = o_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kTmemSlot);
+  volatile int* merge_flag = reinterpret_cast<volatile int*>(smem + S::kTmemSlot + 4);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);  // one arrival per softmax warp
+      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+      mbar_init(&o_empty[t], 4);
+    }
+    mbar_init(mma_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const int D = a.dim;
+  const int tile_tokens = kTensorTileRows / a.group;
+  grid_dependency_wait();  // the plan's lists from here on
+
+  if (kTiles == 2 && warp < 4) setmaxnreg_dec<S::kRegsControl>();
+  if (warp == 0) {
+    // ------------------------------------------------------------------------- TMA producer
+    // Lane l issues the l-th box of a K (or V) tile: boxes x blocks of 64 values, at most 32.
+    if (lane == 0) {
+      tma_prefetch_desc(&qmap);
+      tma_prefetch_desc(&kmap);
+      tma_prefetch_desc(&vmap);
+    }
+    bool ok = true;
+    uint32_t kc = 0, qc = 0;
+    const int boxes = BN / a.box_rows;
+    const int box = lane % boxes, blk = lane / boxes;
+    const uint32_t box_bytes = a.box_rows * 128;
+    const uint32_t q_bytes = static_cast<uint32_t>(tile_tokens) * a.group * 128;
+    auto wait_or_fail = [&](uint64_t* bar, uint32_t parity, int site) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity, a.budget_ns))) {
+        ok = false;
+        if (lane == 0) record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, site);
+      }
+      return ok;
+    };
+    ChunkCursor cur;
+    cursor_init(a, cur);
+    ChunkSegment sg;
+    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, cur, sg)), 0)) {
+      const int n = __shfl_sync(0xffffffffu, sg.n, 0);
+      if (n <= 0) continue;
+      if (wait_or_fail(q_empty, (qc & 1) ^ 1, 80) && lane == 0) {
+        const int tiles_q = kTiles == 2 && sg.count > tile_tokens ? 2 : 1;
+        mbar_arrive_expect_tx(q_full, tiles_q * NB * q_bytes);
+        for (int t = 0; t < tiles_q; ++t) {
+          for (int b = 0; b < NB; ++b) {
+            tma_load_4d(q_smem + t * S::kQBytes + b * S::kTileBytes, &qmap, q_full, b * 64, 0, sg.hk,
+                        sg.token0 + t * tile_tokens);
+          }
+        }
+      }
+      ++qc;
+      const int32_t* table = a.table + static_cast<long long>(sg.b) * a.width;
+      for (int j = 0; j < n; ++j) {
+        const int tok = (sg.n_begin + j) * BN + box * a.box_rows;
+        const bool load = blk < NB && tok < sg.limit;
+        const int row = load ? table[tok / a.page] * a.page + tok % a.page : 0;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box_bytes;
+        const int st = kc % NS;
+        const uint32_t parity = ((kc / NS) & 1) ^ 1;
+        uint8_t* dst = k_smem + st * S::kKVBytes + blk * BN * 128 + box * box_bytes;
+        if (wait_or_fail(&k_empty[st], parity, 81)) {
+          if (lane == 0) mbar_arrive_expect_tx(&k_full[st], bytes);
+          __syncwarp();
+          if (load) tma_load_3d(dst, &kmap, &k_full[st], blk * 64, sg.hk, row);
+        }
+        if (wait_or_fail(&v_empty[st], parity, 82)) {
+          if (lane == 0) mbar_arrive_expect_tx(&v_full[st], bytes);
+          __syncwarp();
+          if (load) tma_load_3d(dst + (S::kV - S::kK), &vmap, &v_full[st], blk * 64, sg.hk, row);
+        }
+        ++kc;
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------------- MMA issuer
+    // The whole warp runs this role converged, its loop state warp-uniform; every tcgen05 issue is predicated on one
+    // elected lane.
+    const uint32_t leader = elect_one_sync();
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+    bool ok = true;
+    uint32_t kc = 0, vc = 0, qc = 0;
+    uint32_t pbits = 0, obits = 0;  // bit t: phase parity of P_t's / O_t's uses
+    const uint32_t idesc_qk = umma_idesc_f16(Tr::kUmmaFormat, 128, BN, 0, 0);
+    const uint32_t idesc_pv = umma_idesc_f16(Tr::kUmmaFormat, 128, D, 0, 1);
+    uint32_t q_lo = umma_desc_lo(smem_u32(q_smem), 16);
+    uint32_t k_lo = umma_desc_lo(smem_u32(k_smem), 16);
+    uint32_t v_lo = umma_desc_lo(smem_u32(v_smem), BN * 128);
+    constexpr uint32_t kHi = umma_desc_hi(1024, 2);
+    const int ksteps = D / 16;
+    auto wait_or_fail = [&](uint64_t* bar, uint32_t parity, int site) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity, a.budget_ns))) {
+        ok = false;
+        if (lane == 0) record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, site);
+      }
+      return ok;
+    };
+    // S_t = Q_t K^T, K from stage st (already waited for)
+    auto qk = [&](int t, int st) {
+      const uint32_t a_lo = q_lo + static_cast<uint32_t>((t * S::kQBytes) >> 4);
+      const uint32_t b_lo = k_lo + static_cast<uint32_t>((st * S::kKVBytes) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < 4 * NB; ++kk) {
+        if (kk < ksteps) {
+          umma_f16_ss_e(leader, tmem_u + S::s_col(t), a_lo + (((kk >> 2) * S::kTileBytes + (kk & 3) * 32) >> 4), kHi,
+                        b_lo + (((kk >> 2) * BN * 128 + (kk & 3) * 32) >> 4), kHi, idesc_qk, kk > 0 ? 1u : 0u);
+        }
+      }
+      umma_commit_e(leader, &s_full[t]);
+    };
+    // O_t += P_t V over 64 keys from step k0 (16 keys each), V from stage st; operands advance through opaque registers
+    // so that the issuer fits its register budget
+    auto pv = [&](int t, int st, bool first, int k0) {
+      uint32_t b_lo = v_lo + static_cast<uint32_t>((st * S::kKVBytes) >> 4) + k0 * ((16 * 128) >> 4);
+      uint32_t p_col = tmem_u + S::s_col(t) + k0 * 8;
+      const uint32_t o_tmem = tmem_u + S::o_col(t);
+#pragma unroll
+      for (int kk = k0; kk < k0 + BN / 32; ++kk) {
+        umma_f16_ts_e(leader, o_tmem, p_col, b_lo, kHi, idesc_pv, (!first || kk > 0) ? 1u : 0u);
+        p_col += 8;
+        b_lo += (16 * 128) >> 4;
+        asm volatile("" : "+r"(p_col), "+r"(b_lo));
+      }
+    };
+    ChunkCursor cur;
+    cursor_init(a, cur);
+    ChunkSegment sg;
+    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, cur, sg)), 0)) {
+      const int n = __shfl_sync(0xffffffffu, sg.n, 0);
+      const int n_a = __shfl_sync(0xffffffffu, tile_steps(a, sg, 0, tile_tokens), 0);
+      const int n_b = kTiles == 2 ? __shfl_sync(0xffffffffu, tile_steps(a, sg, 1, tile_tokens), 0) : 0;
+      if (n <= 0) continue;
+      int kst = kc % NS;
+      if (wait_or_fail(q_full, qc & 1, 83) && wait_or_fail(&k_full[kst], (kc / NS) & 1, 84)) {
+        tc_fence_after_sync();
+        if (n_a > 0) qk(0, kst);
+        if (n_b > 0) qk(1, kst);
+        umma_commit_e(leader, &k_empty[kst]);
+      }
+      ++qc;
+      ++kc;
+      if (n == 1 && ok) umma_commit_e(leader, q_empty);
+      for (int j = 0; j < n; ++j) {
+        // opaque, so the descriptor sums are formed where they are used
+        asm volatile("" : "+r"(q_lo), "+r"(k_lo), "+r"(v_lo));
+        const int vst = vc % NS;
+        const uint32_t v_par = (vc / NS) & 1;
+        ++vc;
+        const bool more = j + 1 < n;
+        const int knext = kc % NS;
+        const uint32_t k_par = (kc / NS) & 1;
+        bool v_seen = false, k_seen = false;
+#pragma unroll 1
+        for (int t = 0; t < kTiles; ++t) {
+          const int nt = t ? n_b : n_a;
+          const bool pv_t = j < nt;
+          const bool qk_t = more && j + 1 < nt;
+          if (pv_t) {
+            // the buffers first, P, which usually comes last, last
+            if (!v_seen) wait_or_fail(&v_full[vst], v_par, 85);
+            v_seen = true;
+            if (qk_t && !k_seen) {
+              wait_or_fail(&k_full[knext], k_par, 86);
+              k_seen = true;
+            }
+            if (j == 0) wait_or_fail(&o_empty[t], ((obits >> t) & 1) ^ 1, 87);
+            if (wait_or_fail(&p_half[t], (pbits >> t) & 1, 88)) {
+              tc_fence_after_sync();
+              pv(t, vst, j == 0, 0);
+            }
+            if (wait_or_fail(&p_full[t], (pbits >> t) & 1, 89)) {
+              tc_fence_after_sync();
+              pv(t, vst, false, BN / 32);
+              if (j + 1 == nt) umma_commit_e(leader, &pv_done[t]);
+              if (qk_t) qk(t, knext);
+            }
+            pbits ^= 1u << t;
+          }
+        }
+        if (ok) umma_commit_e(leader, &v_empty[vst]);
+        if (more) {
+          if (ok) umma_commit_e(leader, &k_empty[knext]);
+          ++kc;
+          if (j + 2 == n && ok) umma_commit_e(leader, q_empty);  // every QK of this item is now issued
+        }
+      }
+      if (n_a > 0) obits ^= 1u;
+      if (n_b > 0) obits ^= 2u;
+    }
+    if (ok) {
+      umma_commit_e(leader, mma_done);
+      __all_sync(0xffffffffu, mbar_wait(mma_done, 0, a.budget_ns));
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------------- softmax / epilogue
+    // Warps 4-7 own query tile A, warps 8-11 tile B; a warp reaches the TMEM lanes of its quarter (warp % 4).
+    if (kTiles == 2) setmaxnreg_inc<S::kRegsSoftmax>();
+    const int t = (warp - 4) / 4;
+    const int row = (warp % 4) * 32 + lane;
+    const int row_token = row / a.group, row_head = row % a.group;
+    const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + S::s_col(t);
+    const uint32_t o_addr = tmem + lane_base + S::o_col(t);
+    bool ok = true;
+    uint32_t sc = 0, pd = 0, vbase = 0;
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity, int site) {
+      if (ok) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, a.budget_ns));
+        if (!ok && lane == 0) record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, site);
+      }
+      return ok;
+    };
+    ChunkCursor cur;
+    cursor_init(a, cur);
+    ChunkSegment sg;
+    while (next_segment(a, cur, sg)) {
+      const int i_tok = t * tile_tokens + row_token;  // token within the item
+      const bool row_valid = row_token < tile_tokens && i_tok < sg.count;
+      // rows of no token compute on whatever Q's tile holds (rows do not mix) and are never stored
+      const int vis = row_valid ? seen_keys(a, sg, i_tok) : sg.limit;
+      const int n_t = tile_steps(a, sg, t, tile_tokens);
+      const int n_other = t == 0 ? 0 : tile_steps(a, sg, 0, tile_tokens);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n_t; ++j) {
+        const int tok0 = (sg.n_begin + j) * BN;
+        wait_warp(&s_full[t], sc & 1, 90 + t);
+        ++sc;
+        const int valid_cols = min(max(vis - tok0, 0), BN);
+        uint32_t sr[BN];
+        if (ok) {
+          tc_fence_after_sync();
+#pragma unroll
+          for (int cb = 0; cb < BN / 64; ++cb) {
+            tmem_ld64(s_addr + cb * 64, *reinterpret_cast<uint32_t(*)[64]>(&sr[cb * 64]));
+          }
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < BN; ++i) sr[i] = 0xff800000u;
+        }
+        if (valid_cols < BN) {  // ragged or diagonal tile
+#pragma unroll
+          for (int col = 0; col < BN; ++col) {
+            if (col >= valid_cols) sr[col] = 0xff800000u;  // -inf
+          }
+        }
+        auto sval = [&](int col) -> float { return __uint_as_float(sr[col]); };
+        float mq0 = -INFINITY, mq1 = -INFINITY, mq2 = -INFINITY, mq3 = -INFINITY;
+#pragma unroll
+        for (int col = 0; col < BN; col += 8) {
+          mq0 = max3(mq0, sval(col), sval(col + 1));
+          mq1 = max3(mq1, sval(col + 2), sval(col + 3));
+          mq2 = max3(mq2, sval(col + 4), sval(col + 5));
+          mq3 = max3(mq3, sval(col + 6), sval(col + 7));
+        }
+        const float mx = max3(mq0, mq1, fmaxf(mq2, mq3)) * a.scale_log2;  // scale > 0; -inf stays -inf
+        // The maximum moves only when it grows by more than 2^8 (P then stays below 2^8, far inside both types' range),
+        // so O is rarely rescaled.
+        float m_new = j == 0 ? mx : m;
+        float alpha = 1.f;
+        if (__any_sync(0xffffffffu, j > 0 && mx > m + 8.0f)) {
+          m_new = fmaxf(m, mx);
+          alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - m_new);
+          if (ok) {
+            // the commit that published S_t(j) also covers PV_t(j - 1): O_t is stable
+            for (int cb = 0; cb < D / 16; ++cb) {
+              uint32_t r[16];
+              tmem_ld16(o_addr + cb * 16, r);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+              tmem_st16(o_addr + cb * 16, r);
+            }
+          }
+        }
+        const float neg_m = (m_new == -INFINITY) ? 0.f : -m_new;
+        float rowsum = 0.f;
+        // Tiles inside the visible keys release P in two halves; the last one releases both at once, after the V rows
+        // past the end are zeroed.
+        const bool early = tok0 + BN <= sg.limit;
+        if (ok) {
+          const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
+          const float2 negm2 = make_float2(neg_m, neg_m);
+          float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t packed[32];
+            exp2_pack64<Tr>(&sr[half * 64], scale2, negm2, acc, packed);
+            tmem_st32(s_addr + half * 32, packed);
+            if (half == 0 && early) {
+              tmem_wait_st();
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[t]);
+            }
+          }
+          tmem_wait_st();
+          rowsum = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y) + (acc[2].x + acc[2].y) + (acc[3].x + acc[3].y);
+        }
+        // V rows past the last visible key hold whatever the stage or the page holds: the first tile to use the stage
+        // zeroes them before it releases P.
+        if (!early && (t == 0 || j >= n_other)) {
+          const uint32_t vcount = vbase + j;
+          const int vst = vcount % NS;
+          wait_warp(&v_full[vst], (vcount / NS) & 1, 92);
+          if (ok && tok0 + row >= sg.limit) {
+            uint8_t* vrow = v_smem + vst * S::kKVBytes + row * 128;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+              for (int ch = 0; ch < 8; ++ch) {
+                *reinterpret_cast<uint4*>(vrow + blk * BN * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+              }
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (!early || !ok) mbar_arrive(&p_half[t]);
+          mbar_arrive(&p_full[t]);
+        }
+        l = l * alpha + rowsum;
+        m = m_new;
+      }
+      if (sg.n > 0) vbase += sg.n;
+      // epilogue
+      float inv = 0.f;
+      if (n_t > 0) {
+        wait_warp(&pv_done[t], pd & 1, 93);
+        ++pd;
+        inv = l > 0.f ? 1.f / l : 0.f;
+        if (ok) tc_fence_after_sync();
+      }
+      T* out_row = static_cast<T*>(a.out) + (row_valid ? (sg.token0 + i_tok) * a.out_stride : 0) +
+                   static_cast<long long>(sg.hk * a.group + row_head) * D;
+      auto load_o = [&](int cb, float (&o)[16]) {
+        if (n_t > 0 && ok) {
+          uint32_t r[16];
+          tmem_ld16(o_addr + cb * 16, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = l > 0.f ? __uint_as_float(r[i]) * inv : 0.f;  // no key seen: exact zeros
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = 0.f;
+        }
+      };
+      auto store_row = [&](int cb, const float (&o)[16], float scale) {
+        uint4* dst = reinterpret_cast<uint4*>(out_row + cb * 16);
+        dst[0] = make_uint4(Tr::pack2(o[0] * scale, o[1] * scale), Tr::pack2(o[2] * scale, o[3] * scale),
+                            Tr::pack2(o[4] * scale, o[5] * scale), Tr::pack2(o[6] * scale, o[7] * scale));
+        dst[1] = make_uint4(Tr::pack2(o[8] * scale, o[9] * scale), Tr::pack2(o[10] * scale, o[11] * scale),
+                            Tr::pack2(o[12] * scale, o[13] * scale), Tr::pack2(o[14] * scale, o[15] * scale));
+      };
+      if (!sg.piece) {
+        for (int cb = 0; cb < D / 16; ++cb) {
+          float o[16];
+          load_o(cb, o);  // warp-collective: every lane, valid row or not
+          if (row_valid) store_row(cb, o, 1.f);
+        }
+        if (n_t > 0) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[t]);
+        }
+        continue;
+      }
+      // A piece of an item cut between CTAs: FP32 O and base-2 LSE go to its slot (O in groups of four columns,
+      // [D / 4][rows][4], so a warp's rows write 512 contiguous bytes per group), and the piece that completes the set
+      // merges all pieces in their order. No CTA waits for another.
+      constexpr int kSlotRows = kTensorTileRows * kTiles;
+      const int r = kTensorTileRows * t + row;
+      auto slot_group = [&](int slot, int g) -> float4* {
+        return reinterpret_cast<float4*>(a.list.slot_o) + (static_cast<long long>(slot) * (D / 4) + g) * kSlotRows + r;
+      };
+      const ChunkPieces pieces = chunk_pieces(a, sg);
+      const int my_slot = pieces.slot(blockIdx.x);
+      for (int cb = 0; cb < D / 16; ++cb) {
+        float o[16];
+        load_o(cb, o);
+        if (row_valid) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            *slot_group(my_slot, cb * 4 + i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+      }
+      if (row_valid) {
+        a.list.slot_lse[static_cast<long long>(my_slot) * kSlotRows + r] =
+            (n_t > 0 && l > 0.f) ? m + fast_log2(l) : kEmptyLse;
+      }
+      if (n_t > 0) {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[t]);
+      }
+      named_barrier_sync(1, 128 * kTiles);
+      if (warp == 4 && lane == 0) {
+        __threadfence();
+        *merge_flag = atomicAdd(&a.list.counters[pieces.q_first], 1) + 1 == pieces.pieces ? 1 : 0;
+      }
+      named_barrier_sync(1, 128 * kTiles);
+      const int merge = *merge_flag;
+      named_barrier_sync(1, 128 * kTiles);  // read by all before the next write
+      if (merge == 0) continue;
+      __threadfence();
+      if (!row_valid) continue;
+      auto lse_of = [&](int p) { return __ldcg(&a.list.slot_lse[static_cast<long long>(pieces.slot(p)) * kSlotRows + r]); };
+      float peak = kEmptyLse, wsum = 0.f;
+      for (int p = pieces.q_first; p <= pieces.q_last; ++p) {
+        if (pieces.holds(p)) peak = fmaxf(peak, lse_of(p));
+      }
+      auto weight = [&](int p) {
+        const float lse = lse_of(p);
+        return lse > kValidLse ? fast_exp2(lse - peak) : 0.f;
+      };
+      for (int p = pieces.q_first; p <= pieces.q_last; ++p) {
+        if (pieces.holds(p)) wsum += weight(p);
+      }
+      const float scale = wsum > 0.f ? 1.f / wsum : 0.f;
+      // 32 values of every piece per round with independent 16-byte loads
+      for (int cb = 0; cb < D / 16; cb += 2) {
+        const bool second = cb + 1 < D / 16;
+        float acc0[16], acc1[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc0[i] = acc1[i] = 0.f;
+        for (int p = pieces.q_first; p <= pieces.q_last; ++p) {
+          if (!pieces.holds(p)) continue;
+          const float wk = weight(p);
+          if (wk == 0.f) continue;
+          const int slot = pieces.slot(p);
+          float4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = (i < 4 || second) ? __ldcg(slot_group(slot, cb * 4 + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc0[4 * i] = fmaf(wk, v[i].x, acc0[4 * i]);
+            acc0[4 * i + 1] = fmaf(wk, v[i].y, acc0[4 * i + 1]);
+            acc0[4 * i + 2] = fmaf(wk, v[i].z, acc0[4 * i + 2]);
+            acc0[4 * i + 3] = fmaf(wk, v[i].w, acc0[4 * i + 3]);
+            acc1[4 * i] = fmaf(wk, v[4 + i].x, acc1[4 * i]);
+            acc1[4 * i + 1] = fmaf(wk, v[4 + i].y, acc1[4 * i + 1]);
+            acc1[4 * i + 2] = fmaf(wk, v[4 + i].z, acc1[4 * i + 2]);
+            acc1[4 * i + 3] = fmaf(wk, v[4 + i].w, acc1[4 * i + 3]);
+          }
+        }
+        store_row(cb, acc0, scale);
+        if (second) store_row(cb + 1, acc1, scale);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, S::kTmemCols);
+  }
+}
+
+template <typename T, int NB>
+static cudaError_t launch_tensor_t(const fgw_chunk_params& p, ChunkArgs a, int device, cudaStream_t stream) {
+  using S = TensorShape<NB>;
+  auto kernel = chunk_tensor_kernel<T, NB>;
+  int regs = 0;
+  cudaError_t err = prepare_kernel(reinterpret_cast<const void*>(kernel), S::kBytes, device, &regs);
+  if (err != cudaSuccess) return err;
+  // setmaxnreg.inc draws on the registers the block was launched with: refuse a build that would not cover the split
+  const int allocated = ((regs + 7) / 8) * 8 * S::kThreads;
+  if (S::kTiles == 2 && allocated < 4 * 32 * S::kRegsControl + 8 * 32 * S::kRegsSoftmax) return cudaErrorNotSupported;
+  a.box_rows = chunk_box_rows(p.page_size, S::kBN);
+  CUtensorMap qmap, kmap, vmap;
+  // a tile's rows: all heads of the group, token by token
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.head_dim), static_cast<cuuint64_t>(a.group),
+                              static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.tokens)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.head_dim) * 2,
+                                 static_cast<cuuint64_t>(p.head_dim) * a.group * 2,
+                                 static_cast<cuuint64_t>(p.q_stride) * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(a.group), 1,
+                             static_cast<cuuint32_t>(kTensorTileRows / a.group)};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type =
+      p.dtype == FGW_DTYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (encode_tiled_cached(&qmap, type, 4, const_cast<void*>(p.q), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    return cudaErrorInvalidValue;
+  }
+  if (chunk_kv_map(&kmap, p, p.k_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
+  if (chunk_kv_map(&vmap, p, p.v_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
+  return launch_after_plan(kernel, static_cast<unsigned>(a.programs), S::kThreads, S::kBytes, stream, qmap, kmap, vmap,
+                           a);
+}
+
+template <typename T>
+static cudaError_t launch_tensor_nb(const fgw_chunk_params& p, const ChunkArgs& a, int device, cudaStream_t stream) {
+  switch ((p.head_dim + 63) / 64) {
+    case 1:
+      return launch_tensor_t<T, 1>(p, a, device, stream);
+    case 2:
+      return launch_tensor_t<T, 2>(p, a, device, stream);
+    case 3:
+      return launch_tensor_t<T, 3>(p, a, device, stream);
+    default:
+      return launch_tensor_t<T, 4>(p, a, device, stream);
+  }
+}
+
+cudaError_t launch_chunk_tensor(const fgw_chunk_params& p, ChunkArgs a, int device, cudaStream_t stream) {
+  return p.dtype == FGW_DTYPE_BFLOAT16 ? launch_tensor_nb<__nv_bfloat16>(p, a, device, stream)
+                                       : launch_tensor_nb<__half>(p, a, device, stream);
+}
+
+}  // namespace fgw
