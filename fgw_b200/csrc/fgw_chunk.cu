@@ -8,7 +8,8 @@
 // rows per key head to the decode kernel (fgw_chunk_decode.cu, bound by HBM), the others to the tensor kernel
 // (fgw_chunk_sm100.cu, tcgen05). Lengths are device data, so the host does not know which requests are which: with at
 // most 16 rows per request on average it launches the decode kernel alone, which then takes everything (a longer
-// request in several items), else both, in the order plan, decode, tensor.
+// request in several items), else both. The plan (tensor kernel only), decode, tensor and merge kernels follow one
+// another as programmatic dependent launches, so each one's set-up overlaps the one before.
 #include <algorithm>
 #include <numeric>
 
@@ -17,16 +18,11 @@
 namespace fgw {
 
 constexpr int kPlanListThreads = 1024;
-constexpr int kPlanSorted = 2048;  // rows of a list sorted in shared memory; longer lists keep the request order
-
-enum ChunkClass { kDecodeList = 0, kTensorList = 1 };
-
-struct ChunkPlanArgs {
-  ChunkArgs a[2];   // by class; only the lists differ
-  bool on[2];
-  bool split;       // requests go by their rows; otherwise everything is the decode list's
-  int row_bytes;    // of an output row
-};
+constexpr int kPlanSorted = 2048;     // rows of a list sorted in shared memory; longer lists keep the request order
+constexpr int kItemCost = 2;          // KV tiles that an item's start and end cost, in the choice of whole rounds
+constexpr int kTensorMinUnits = 2;    // units a program's range has at least when every item is cut
+constexpr int kMergeThreads = 256;
+constexpr int kMergeRows = 32;        // rows merged by one CTA
 
 // Sum over the CTA of each thread's value before it in thread order, and the total.
 template <typename V>
@@ -55,139 +51,275 @@ __device__ __forceinline__ V block_scan(V v, V& total, V* shared) {
   return sum - v + (warp > 0 ? shared[warp - 1] : V(0));
 }
 
-__global__ void __launch_bounds__(kPlanListThreads) chunk_plan_kernel(const __grid_constant__ ChunkPlanArgs plan) {
-  grid_dependents_launch();
-  __shared__ long long scan_l[32];
-  __shared__ int scan_i[32];
-  __shared__ int units_s[kPlanSorted];
-  const int cls = plan.on[kDecodeList] ? static_cast<int>(blockIdx.x) : kTensorList;
-  const ChunkArgs& a = plan.a[cls];
-  const ChunkList& list = a.list;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (blockIdx.x == 0 && tid == 0) {
-    a.ws->error = 0;
-    a.ws->error_site = 0;
-  }
-  for (int p = tid; p < a.programs; p += kPlanListThreads) list.counters[p] = 0;
+// The tensor kernel's work list: the items by descending units; whole rounds of one item per program in snake order,
+// either all of them, where that comes within 5 % and four tiles of an equal share, or as many as stay within each
+// program's share, the rest cut into a contiguous range of units per program that fills its share up.
+struct PlanShared {
+  long long scan_l[32];
+  int scan_i[32];
+  int4 raw[kPlanSorted], rows[kPlanSorted];
+  long long prefix[kPlanSorted + 1];
+  int first[kPlanSorted + 1];
+};
 
-  // rows of each request, and their place in the list
-  auto rows_of = [&](int b) {
-    const NewTokens nt = new_tokens(a.cu, a.tokens, b);
-    const bool small = nt.count * a.group <= kDecodeRows;
-    if (plan.split && small != (cls == kDecodeList)) return 0;
-    return (nt.count + list.tokens_per_item - 1) / list.tokens_per_item;
-  };
+__global__ void __launch_bounds__(kPlanListThreads)
+    chunk_plan_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ ChunkList list) {
+  grid_dependents_launch();
+  extern __shared__ uint8_t plan_smem[];
+  PlanShared& sh = *reinterpret_cast<PlanShared*>(plan_smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // rows of each request, and their place in the list; lists that fit stay in shared memory
+  int* first = a.batch <= kPlanSorted ? sh.first : list.first;
   int rows = 0;
   for (int base = 0; base < a.batch; base += kPlanListThreads) {
     const int b = base + tid;
     int all;
-    const int at = block_scan(b < a.batch ? rows_of(b) : 0, all, scan_i);
-    if (b < a.batch) list.first[b] = rows + at;
+    const int mine = b < a.batch ? item_rows(a, new_tokens(a.cu, a.tokens, b).count, false) : 0;
+    const int at = block_scan(mine, all, sh.scan_i);
+    if (b < a.batch) first[b] = rows + at;
     rows += all;
   }
   rows = min(rows, list.max_rows);
-  if (tid == 0) list.first[a.batch] = rows;
+  if (tid == 0) first[a.batch] = rows;
   __syncthreads();
+  const bool small = rows <= kPlanSorted;
+  int4* raw = small ? sh.raw : list.unsorted;
   for (int b = warp; b < a.batch; b += kPlanListThreads / 32) {
-    const int begin = min(list.first[b], rows), end = min(list.first[b + 1], rows);
+    const int begin = min(first[b], rows), end = min(first[b + 1], rows);
     if (begin >= end) continue;
-    const NewTokens nt = new_tokens(a.cu, a.tokens, b);
+    const int count = new_tokens(a.cu, a.tokens, b).count;
     const int len = held_tokens(a.lens, b, a.width, a.page);
     for (int r = begin + lane; r < end; r += 32) {
-      const int t0 = (r - begin) * list.tokens_per_item;
-      const int last = min(t0 + list.tokens_per_item, nt.count) - 1;
-      const int seen = max(a.causal ? len - nt.count + last + 1 : len, 0);
-      const int units = max((seen + list.keys_per_unit - 1) / list.keys_per_unit, 1);  // no keys: zeros to write
-      list.unsorted[r] = make_int4(b, t0, units, 0);
-      if (r < kPlanSorted) units_s[r] = units;
+      const int t0 = (r - begin) * a.tokens_per_item;
+      raw[r] = make_int4(b, t0, item_units(a, count, len, t0), 0);
     }
   }
   __syncthreads();
-  // by descending units (ties: in order), so that whole items are dealt longest first
+  // by descending units (ties: in order), so that whole items are dealt longest first; with fewer items than programs
+  // all are cut and the order does not matter
+  const int programs = a.programs;
   const int items = rows * a.kv_heads;
-  const bool sorted = rows <= kPlanSorted;
-  const bool order = sorted && items >= a.programs;
+  const bool order = small && items > programs;
+  int4* sorted = small ? sh.rows : list.rows;
   for (int r = tid; r < rows; r += kPlanListThreads) {
-    const int4 row = list.unsorted[r];
+    const int4 row = raw[r];
     int rank = r;
     if (order) {
       rank = 0;
-      for (int s = 0; s < rows; ++s) rank += (units_s[s] > row.z || (units_s[s] == row.z && s < r)) ? 1 : 0;
+      for (int s = 0; s < rows; ++s) rank += (raw[s].z > row.z || (raw[s].z == row.z && s < r)) ? 1 : 0;
     }
-    list.rows[rank] = row;
+    sorted[rank] = row;
+    if (small) list.rows[rank] = row;
   }
   __syncthreads();
+  long long* prefix = small ? sh.prefix : list.prefix;
   long long total = 0;
   for (int base = 0; base < rows; base += kPlanListThreads) {
     const int r = base + tid;
-    const int units = r < rows ? list.rows[r].z : 0;
-    if (sorted && r < rows) units_s[r] = units;
     long long all;
-    const long long at = block_scan(static_cast<long long>(units) * a.kv_heads, all, scan_l);
-    if (r < rows) list.prefix[r] = total + at;
+    const long long at = block_scan(r < rows ? static_cast<long long>(sorted[r].z) * a.kv_heads : 0ll, all, sh.scan_l);
+    if (r < rows) prefix[r] = total + at;
     total += all;
   }
-  if (tid == 0) list.prefix[rows] = total;
+  if (tid == 0) prefix[rows] = total;
   __syncthreads();
-  // whole rounds in snake order while every program stays within its share
-  const int programs = a.programs;
   const bool mine = tid < programs;
-  const long long share = mine ? program_start(total, programs, tid + 1) - program_start(total, programs, tid) : 0;
+  auto units_of = [&](int round) {  // of this program's item in a round, 0 when it has none
+    const int item = round * programs + ((round & 1) ? programs - 1 - tid : tid);
+    return mine && item < items ? sorted[item / a.kv_heads].z : 0;
+  };
+  const int all_rounds = (items + programs - 1) / programs;
+  int rounds = 0, ranges = programs;
   long long load = 0;
-  int rounds = 0;
-  while (static_cast<long long>(rounds + 1) * programs <= items) {
-    const int item = rounds * programs + ((rounds & 1) ? programs - 1 - tid : tid);
-    int units = 0;
-    if (mine) units = sorted ? units_s[item / a.kv_heads] : list.rows[item / a.kv_heads].z;
-    if (!__syncthreads_and(!mine || load + units <= share)) break;
-    load += units;
-    ++rounds;
-  }
-  long long rest;
-  const long long before = block_scan(mine ? share - load : 0ll, rest, scan_l);
-  const int cut = rounds * programs;  // first cut item
-  const int cut_row = cut / a.kv_heads;
-  long long cut_u = total;
-  if (cut < items) {
-    cut_u = list.prefix[cut_row] + static_cast<long long>(cut % a.kv_heads) * list.rows[cut_row].z;
-  }
-  if (mine) {
-    const long long u = cut_u + before;
-    list.prog_u[tid] = u;
-    if (tid == programs - 1) list.prog_u[programs] = total;
-    int lo = 0, hi = max(rows - 1, 0);
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (list.prefix[mid] <= u) {
-        lo = mid;
-      } else {
-        hi = mid - 1;
+  if (items > programs) {
+    for (int r = 0; r < all_rounds; ++r) {
+      const int units = units_of(r);
+      load += units > 0 ? units + kItemCost : 0;
+    }
+    const long long equal = (total + static_cast<long long>(items) * kItemCost) / programs;
+    if (__syncthreads_and(load <= equal + equal / 20 + 4)) {
+      rounds = all_rounds;
+    } else {
+      const long long share = mine ? program_start(total, programs, tid + 1) - program_start(total, programs, tid) : 0;
+      load = 0;
+      while (static_cast<long long>(rounds + 1) * programs <= items) {
+        const int units = units_of(rounds);
+        if (!__syncthreads_and(!mine || load + units <= share)) break;
+        load += units;
+        ++rounds;
       }
     }
+  } else {
+    ranges = static_cast<int>(max(1ll, min(static_cast<long long>(programs), total / kTensorMinUnits)));
+  }
+  const int cut = min(rounds * programs, items);  // first cut item
+  const bool none = cut == items;
+  long long share = 0;
+  if (!none && rounds > 0) {
+    share = program_start(total, programs, tid + 1) - program_start(total, programs, tid) - load;
+  } else if (!none && tid < ranges) {
+    share = program_start(total, ranges, tid + 1) - program_start(total, ranges, tid);
+  }
+  long long rest;
+  const long long before = block_scan(mine ? share : 0ll, rest, sh.scan_l);
+  if (mine) {
+    long long u = total;
     int item = 0, off = 0;
-    if (rows > 0 && u < total) {
-      const int units = list.rows[lo].z;
-      const long long within = u - list.prefix[lo];
-      item = lo * a.kv_heads + static_cast<int>(within / units);
-      off = static_cast<int>(within % units);
+    if (!none) {
+      const int cut_row = cut / a.kv_heads;
+      u = prefix[cut_row] + static_cast<long long>(cut % a.kv_heads) * sorted[cut_row].z + before;
+      int lo = 0, hi = rows - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (prefix[mid] <= u) {
+          lo = mid;
+        } else {
+          hi = mid - 1;
+        }
+      }
+      if (u < total) {
+        const int units = sorted[lo].z;
+        const long long within = u - prefix[lo];
+        item = lo * a.kv_heads + static_cast<int>(within / units);
+        off = static_cast<int>(within % units);
+      }
     }
+    list.prog_u[tid] = u;
     list.prog_item[tid] = item;
     list.prog_off[tid] = off;
   }
   if (tid == 0) {
+    list.prog_u[programs] = total;
     list.meta->items = items;
     list.meta->rounds = rounds;
+  }
+}
+
+// Merges the pieces of the cut items of both kernels, kMergeRows rows per CTA: the weights 2^(lse - peak) of all pieces
+// first, in shared memory, then the weighted sum of their O in piece order with independent loads. Also writes zeros
+// into the rows of no request and reduces the CTAs' errors to the header's word.
+struct MergeList {
+  ChunkSlots slots;
+  const long long* prog_u;  // [programs + 1]: programs without units hold no piece (nullptr: all hold one)
+  int slot_rows, parts;     // parts CTAs per program
+  bool by_column;           // O laid out [dim / 4][rows][4], else [rows][dim]
+};
+struct MergeArgs {
+  ChunkArgs a;
+  WorkspaceHeader* ws;
+  MergeList list[2];  // decode, tensor; parts 0: kernel not launched
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid_constant__ MergeArgs m) {
+  using Tr = ElemTraits<T>;
+  __shared__ float weight[kStreamMaxPrograms][kMergeRows];
+  __shared__ float inverse[kMergeRows];
+  __shared__ int slot[kStreamMaxPrograms];
+  __shared__ int pieces_s;
+  const ChunkArgs& a = m.a;
+  grid_dependency_wait();
+  const int tid = threadIdx.x;
+  if (blockIdx.x == 0 && tid < 32) {
+    int code = 0, site = 0;
+    for (int k = 0; k < 2; ++k) {
+      for (int p = tid; m.list[k].parts > 0 && p < a.programs; p += 32) {
+        const int2 e = m.list[k].slots.errors[p];
+        if (e.x != 0 && code == 0) {
+          code = e.x;
+          site = e.y;
+        }
+      }
+    }
+    const uint32_t any = __ballot_sync(0xffffffffu, code != 0);
+    const int from = any != 0 ? __ffs(any) - 1 : 0;
+    code = __shfl_sync(0xffffffffu, code, from);
+    site = __shfl_sync(0xffffffffu, site, from);
+    if (tid == 0) {
+      m.ws->error = code;
+      m.ws->error_site = site;
+    }
   }
   // rows of no request
   const long long first = min(max(static_cast<long long>(a.cu[0]), 0ll), a.tokens);
   const long long end = min(max(static_cast<long long>(a.cu[a.batch]), first), a.tokens);
-  const int chunks = plan.row_bytes / 16;
-  const long long none = first + a.tokens - end;
-  for (long long i = static_cast<long long>(blockIdx.x) * kPlanListThreads + tid; i < none * chunks;
-       i += static_cast<long long>(gridDim.x) * kPlanListThreads) {
+  const int chunks = a.heads * a.dim / 8;
+  const long long none = (first + a.tokens - end) * chunks;
+  for (long long i = static_cast<long long>(blockIdx.x) * kMergeThreads + tid; i < none;
+       i += static_cast<long long>(gridDim.x) * kMergeThreads) {
     const long long k = i / chunks;
     const long long t = k < first ? k : end + k - first;
     reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + t * a.out_stride)[i % chunks] = make_uint4(0, 0, 0, 0);
+  }
+  const int decode_ctas = m.list[0].parts * a.programs;
+  const int kind = static_cast<int>(blockIdx.x) < decode_ctas ? 0 : 1;
+  const MergeList& l = m.list[kind];
+  const int at = blockIdx.x - (kind ? decode_ctas : 0);
+  const int q = at / l.parts, row0 = at % l.parts * kMergeRows;
+  const ChunkCut cut = l.slots.cuts[q];
+  // rows of the slot are (tile, row of the tile) for the tensor kernel: tile 1 starts at row 128 whatever the group
+  const int tile_rows = kTensorTileRows / a.group * a.group;
+  if (cut.last < q) return;
+  if (tid == 0) {
+    int n = 0;
+    for (int p = q; p <= cut.last; ++p) {
+      if (l.prog_u == nullptr || l.prog_u[p] < l.prog_u[p + 1]) slot[n++] = 2 * p + (p == q ? 1 : 0);
+    }
+    pieces_s = n;
+  }
+  __syncthreads();
+  const int pieces = pieces_s;
+  for (int i = tid; i < pieces * kMergeRows; i += kMergeThreads) {
+    const int k = i / kMergeRows, r = i % kMergeRows;
+    const bool in = row0 + r < l.slot_rows;
+    weight[k][r] = in ? l.slots.lse[static_cast<long long>(slot[k]) * l.slot_rows + row0 + r] : kEmptyLse;
+  }
+  __syncthreads();
+  if (tid < kMergeRows) {
+    float peak = kEmptyLse, sum = 0.f;
+    for (int k = 0; k < pieces; ++k) peak = fmaxf(peak, weight[k][tid]);
+    for (int k = 0; k < pieces; ++k) {
+      const float lse = weight[k][tid];
+      const float w = lse > kValidLse ? fast_exp2(lse - peak) : 0.f;
+      weight[k][tid] = w;
+      sum += w;
+    }
+    inverse[tid] = sum > 0.f ? 1.f / sum : 0.f;
+  }
+  __syncthreads();
+  const int groups = a.dim / 4;
+  for (int i = tid; i < kMergeRows * groups; i += kMergeThreads) {
+    // neighbouring threads read neighbouring 16 bytes of the slot
+    const int r = l.by_column ? i % kMergeRows : i / groups, g = l.by_column ? i / kMergeRows : i % groups;
+    const int row = row0 + r;
+    const int tile = row / kTensorTileRows, in_tile = row % kTensorTileRows;
+    const int token = tile * (kTensorTileRows / a.group) + in_tile / a.group;
+    if (row >= l.slot_rows || in_tile >= tile_rows || token >= cut.count) continue;
+    const long long step = static_cast<long long>(l.slot_rows) * groups;  // float4s of a slot
+    const float4* src = reinterpret_cast<const float4*>(l.slots.o) +
+                        (l.by_column ? static_cast<long long>(g) * l.slot_rows + row : static_cast<long long>(row) * groups + g);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < pieces; k0 += 8) {
+      float4 v[8];
+      float w[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        w[u] = k0 + u < pieces ? weight[k0 + u][r] : 0.f;
+        v[u] = w[u] != 0.f ? src[slot[k0 + u] * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        acc.x = fmaf(w[u], v[u].x, acc.x);
+        acc.y = fmaf(w[u], v[u].y, acc.y);
+        acc.z = fmaf(w[u], v[u].z, acc.z);
+        acc.w = fmaf(w[u], v[u].w, acc.w);
+      }
+    }
+    const float inv = inverse[r];
+    T* out = static_cast<T*>(a.out) + (cut.token0 + token) * a.out_stride +
+             static_cast<long long>(cut.hk * a.group + in_tile % a.group) * a.dim + g * 4;
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2(Tr::pack2(acc.x * inv, acc.y * inv), Tr::pack2(acc.z * inv, acc.w * inv));
   }
 }
 
@@ -246,87 +378,111 @@ static bool tensor_on(const fgw_chunk_params& p) {
   return !decode_on(p) || p.tokens * (p.heads / p.kv_heads) > static_cast<long long>(kDecodeRows) * p.batch;
 }
 
-// The work list of one class at `at` (sizes alone when at is null); returns the bytes it takes.
-static size_t carve_list(const fgw_chunk_params& p, int cls, uint8_t* at, ChunkList* out) {
+// The workspace from `at` on (sizes alone when it is null), by class: slots of both kernels, the tensor kernel's list.
+struct ChunkLayout {
+  ChunkSlots slots[2];
+  int tokens_per_item[2], keys_per_unit[2], slot_rows[2];
+  ChunkList list;
+  size_t bytes;
+};
+
+static ChunkLayout chunk_layout(const fgw_chunk_params& p, uint8_t* const begin) {
   const int group = p.heads / p.kv_heads, nb = (p.head_dim + 63) / 64;
-  ChunkList l;
-  int slot_rows;
-  if (cls == kDecodeList) {
-    l.tokens_per_item = kDecodeRows / group;
-    l.keys_per_unit = chunk_decode_keys(nb);
-    slot_rows = kDecodeRows;
-  } else {
-    l.tokens_per_item = kTensorTileRows / group * chunk_tensor_tiles(nb);
-    l.keys_per_unit = 128;
-    slot_rows = kTensorTileRows * chunk_tensor_tiles(nb);
-  }
-  l.max_rows = static_cast<int>(p.tokens / l.tokens_per_item + p.batch);
-  uint8_t* const begin = at;
+  ChunkLayout l = {};
+  uint8_t* at = begin;
   auto take = [&](size_t n) {
     uint8_t* here = at;
     at += (n + 255) & ~size_t(255);
     return here;
   };
-  const size_t rows = l.max_rows, programs = kStreamMaxPrograms;
-  l.meta = reinterpret_cast<ChunkMeta*>(take(sizeof(ChunkMeta)));
-  l.rows = reinterpret_cast<int4*>(take(rows * sizeof(int4)));
-  l.unsorted = reinterpret_cast<int4*>(take(rows * sizeof(int4)));
-  l.prefix = reinterpret_cast<long long*>(take((rows + 1) * 8));
-  l.first = reinterpret_cast<int32_t*>(take((static_cast<size_t>(p.batch) + 1) * 4));
-  l.prog_item = reinterpret_cast<int32_t*>(take(programs * 4));
-  l.prog_off = reinterpret_cast<int32_t*>(take(programs * 4));
-  l.prog_u = reinterpret_cast<long long*>(take((programs + 1) * 8));
-  l.counters = reinterpret_cast<int32_t*>(take(programs * 4));
-  l.slot_lse = reinterpret_cast<float*>(take(2 * programs * slot_rows * 4));
-  l.slot_o = reinterpret_cast<float*>(take(2 * programs * slot_rows * static_cast<size_t>(p.head_dim) * 4));
-  if (out != nullptr) *out = l;
-  return static_cast<size_t>(at - begin);
+  take(sizeof(WorkspaceHeader));
+  const size_t programs = kStreamMaxPrograms;
+  const bool on[2] = {decode_on(p), tensor_on(p)};
+  l.tokens_per_item[0] = kDecodeRows / group;
+  l.keys_per_unit[0] = chunk_decode_keys(nb);
+  l.slot_rows[0] = kDecodeRows;
+  l.tokens_per_item[1] = kTensorTileRows / group * chunk_tensor_tiles(nb);
+  l.keys_per_unit[1] = 128;
+  l.slot_rows[1] = kTensorTileRows * chunk_tensor_tiles(nb);
+  for (int k = 0; k < 2; ++k) {
+    if (!on[k]) continue;
+    l.slots[k].cuts = reinterpret_cast<ChunkCut*>(take(programs * sizeof(ChunkCut)));
+    l.slots[k].errors = reinterpret_cast<int2*>(take(programs * sizeof(int2)));
+    l.slots[k].lse = reinterpret_cast<float*>(take(2 * programs * l.slot_rows[k] * 4));
+    l.slots[k].o = reinterpret_cast<float*>(take(2 * programs * l.slot_rows[k] * static_cast<size_t>(p.head_dim) * 4));
+  }
+  if (on[1]) {
+    ChunkList& w = l.list;
+    w.max_rows = static_cast<int>(p.tokens / l.tokens_per_item[1] + p.batch);
+    const size_t rows = w.max_rows;
+    w.meta = reinterpret_cast<ChunkMeta*>(take(sizeof(ChunkMeta)));
+    w.rows = reinterpret_cast<int4*>(take(rows * sizeof(int4)));
+    w.unsorted = reinterpret_cast<int4*>(take(rows * sizeof(int4)));
+    w.prefix = reinterpret_cast<long long*>(take((rows + 1) * 8));
+    w.first = reinterpret_cast<int32_t*>(take((static_cast<size_t>(p.batch) + 1) * 4));
+    w.prog_item = reinterpret_cast<int32_t*>(take(programs * 4));
+    w.prog_off = reinterpret_cast<int32_t*>(take(programs * 4));
+    w.prog_u = reinterpret_cast<long long*>(take((programs + 1) * 8));
+  }
+  l.bytes = static_cast<size_t>(at - begin);
+  return l;
 }
 
-size_t chunk_workspace_bytes(const fgw_chunk_params& p) {
-  size_t bytes = sizeof(WorkspaceHeader);
-  if (decode_on(p)) bytes += carve_list(p, kDecodeList, nullptr, nullptr);
-  if (tensor_on(p)) bytes += carve_list(p, kTensorList, nullptr, nullptr);
-  return bytes;
-}
+size_t chunk_workspace_bytes(const fgw_chunk_params& p) { return chunk_layout(p, nullptr).bytes; }
 
 cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_count, int device, cudaStream_t stream) {
-  ChunkPlanArgs plan = {};
-  plan.on[kDecodeList] = decode_on(p);
-  plan.on[kTensorList] = tensor_on(p);
-  plan.split = plan.on[kDecodeList] && plan.on[kTensorList];
-  plan.row_bytes = p.heads * p.head_dim * 2;
-  ChunkArgs a = {};
-  a.out = p.out;
-  a.table = p.block_table;
-  a.lens = p.cache_seqlens;
-  a.cu = p.cu_seqlens_q;
-  a.q = p.q;
-  a.ws = static_cast<WorkspaceHeader*>(workspace);
-  a.tokens = p.tokens;
-  a.q_stride = p.q_stride;
-  a.out_stride = p.out_stride;
-  a.batch = p.batch;
-  a.heads = p.heads;
-  a.kv_heads = p.kv_heads;
-  a.group = p.heads / p.kv_heads;
-  a.dim = p.head_dim;
-  a.width = p.table_width;
-  a.page = p.page_size;
-  a.causal = p.causal;
-  a.programs = std::min(sm_count, kStreamMaxPrograms);
-  a.scale_log2 = p.softmax_scale * kLog2e;
-  a.budget_ns = static_cast<uint64_t>(p.wait_budget_ms > 0 ? p.wait_budget_ms : 2000) * 1000000ull;
-  uint8_t* at = static_cast<uint8_t*>(workspace) + sizeof(WorkspaceHeader);
-  for (int cls = 0; cls < 2; ++cls) {
-    plan.a[cls] = a;
-    if (plan.on[cls]) at += carve_list(p, cls, at, &plan.a[cls].list);
+  const ChunkLayout layout = chunk_layout(p, static_cast<uint8_t*>(workspace));
+  const bool on[2] = {decode_on(p), tensor_on(p)};
+  ChunkArgs a[2] = {};
+  a[0].out = p.out;
+  a[0].table = p.block_table;
+  a[0].lens = p.cache_seqlens;
+  a[0].cu = p.cu_seqlens_q;
+  a[0].q = p.q;
+  a[0].tokens = p.tokens;
+  a[0].q_stride = p.q_stride;
+  a[0].out_stride = p.out_stride;
+  a[0].batch = p.batch;
+  a[0].heads = p.heads;
+  a[0].kv_heads = p.kv_heads;
+  a[0].group = p.heads / p.kv_heads;
+  a[0].dim = p.head_dim;
+  a[0].width = p.table_width;
+  a[0].page = p.page_size;
+  a[0].causal = p.causal;
+  a[0].programs = std::min(sm_count, kStreamMaxPrograms);
+  a[0].split = on[0] && on[1] ? 1 : 0;
+  a[0].scale_log2 = p.softmax_scale * kLog2e;
+  a[0].budget_ns = static_cast<uint64_t>(p.wait_budget_ms > 0 ? p.wait_budget_ms : 2000) * 1000000ull;
+  a[1] = a[0];
+  MergeArgs merge = {};
+  merge.ws = static_cast<WorkspaceHeader*>(workspace);
+  for (int k = 0; k < 2; ++k) {
+    a[k].tokens_per_item = layout.tokens_per_item[k];
+    a[k].keys_per_unit = layout.keys_per_unit[k];
+    a[k].slots = layout.slots[k];
+    if (!on[k]) continue;
+    merge.list[k].slots = layout.slots[k];
+    merge.list[k].slot_rows = layout.slot_rows[k];
+    merge.list[k].parts = (layout.slot_rows[k] + kMergeRows - 1) / kMergeRows;
+    merge.list[k].by_column = k == 1;
+    merge.list[k].prog_u = k == 1 ? layout.list.prog_u : nullptr;
   }
-  chunk_plan_kernel<<<plan.split ? 2 : 1, kPlanListThreads, 0, stream>>>(plan);
-  cudaError_t err = cudaGetLastError();
-  if (err == cudaSuccess && plan.on[kDecodeList]) err = launch_chunk_decode(p, plan.a[kDecodeList], device, stream);
-  if (err == cudaSuccess && plan.on[kTensorList]) err = launch_chunk_tensor(p, plan.a[kTensorList], device, stream);
-  return err;
+  merge.a = a[0];
+  cudaError_t err = cudaSuccess;
+  if (on[1]) {
+    err = prepare_kernel(reinterpret_cast<const void*>(chunk_plan_kernel), sizeof(PlanShared), device, nullptr);
+    if (err != cudaSuccess) return err;
+    chunk_plan_kernel<<<1, kPlanListThreads, sizeof(PlanShared), stream>>>(a[1], layout.list);
+    err = cudaGetLastError();
+  }
+  if (err == cudaSuccess && on[0]) err = launch_chunk_decode(p, a[0], device, stream);
+  if (err == cudaSuccess && on[1]) err = launch_chunk_tensor(p, a[1], layout.list, device, stream);
+  if (err != cudaSuccess) return err;
+  const unsigned grid = static_cast<unsigned>(a[0].programs * (merge.list[0].parts + merge.list[1].parts));
+  return p.dtype == FGW_DTYPE_BFLOAT16
+             ? launch_after_plan(chunk_merge_kernel<__nv_bfloat16>, grid, kMergeThreads, 0, stream, merge)
+             : launch_after_plan(chunk_merge_kernel<__half>, grid, kMergeThreads, 0, stream, merge);
 }
 
 }  // namespace fgw

@@ -9,6 +9,9 @@
 // units of a tile this small would sit idle in tcgen05's 128-row form: 16 rows leave seven eighths of it empty, and
 // its scores would cross TMEM twice.
 //
+// The work is split without a plan kernel: every CTA sums the units of all requests and finds the start of its own
+// range. That costs two or three trips to L2 before the first load; a plan launch ahead of it measured 6 us more.
+//
 // Rows of V from the last visible key on hold whatever the ring or the page holds: the warp zeroes them, since a zero
 // weight times NaN would still be NaN.
 #include <algorithm>
@@ -16,6 +19,8 @@
 #include "fgw_chunk.cuh"
 
 namespace fgw {
+
+constexpr int kDecodeMinUnits = 2;  // units a program takes at least: a piece costs a merge
 
 template <int NB>
 struct DecodeShape {
@@ -64,6 +69,103 @@ __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A CTA's range of units of all items, laid out by request, row and key head.
+struct DecodeCursor {
+  int b, row, hk, off;   // next item and the units of it before the range
+  long long u, u_end;    // units left
+  long long total;       // units of all items, over so many programs
+  int programs;
+};
+
+// Units of request b's items for one key head.
+__device__ __forceinline__ long long request_units(const ChunkArgs& a, int b) {
+  const NewTokens nt = new_tokens(a.cu, a.tokens, b);
+  const int rows = item_rows(a, nt.count, true);
+  const int len = held_tokens(a.lens, b, a.width, a.page);
+  long long units = 0;
+  for (int r = 0; r < rows; ++r) units += item_units(a, nt.count, len, r * a.tokens_per_item);
+  return units;
+}
+
+// Thread t takes the t-th of kThreads equal runs of requests, so one sum over the CTA gives the total and one over the
+// threads before it the run that holds the range's start, which its thread then walks.
+template <int kThreads>
+__device__ DecodeCursor decode_cursor(const ChunkArgs& a, long long* shared, DecodeCursor* found) {
+  const int run = (a.batch + kThreads - 1) / kThreads;
+  const int begin = min(static_cast<int>(threadIdx.x) * run, a.batch), end = min(begin + run, a.batch);
+  long long mine = 0;
+  for (int b = begin; b < end; ++b) mine += request_units(a, b);
+  mine *= a.kv_heads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long before = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += up;
+  }
+  if (lane == 31) shared[warp] = before;
+  if (threadIdx.x == 0) found->u = found->u_end = 0;
+  __syncthreads();
+  long long total = 0, base = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w == warp) base = total;
+    total += shared[w];
+  }
+  before += base - mine;  // units of the runs before this one
+  const int programs = static_cast<int>(max(1ll, min(static_cast<long long>(a.programs), total / kDecodeMinUnits)));
+  const int p = blockIdx.x;
+  if (p < programs) {
+    const long long u = program_start(total, programs, p), u_end = program_start(total, programs, p + 1);
+    if (u < u_end && before <= u && u < before + mine) {
+      long long left = u - before;
+      int b = begin;
+      long long units = request_units(a, b);
+      while (left >= units * a.kv_heads) {
+        left -= units * a.kv_heads;
+        units = request_units(a, ++b);
+      }
+      const NewTokens nt = new_tokens(a.cu, a.tokens, b);
+      const int len = held_tokens(a.lens, b, a.width, a.page);
+      int row = 0;
+      long long w = item_units(a, nt.count, len, 0);
+      while (left >= w * a.kv_heads) {
+        left -= w * a.kv_heads;
+        ++row;
+        w = item_units(a, nt.count, len, row * a.tokens_per_item);
+      }
+      *found = {b, row, static_cast<int>(left / w), static_cast<int>(left % w), u, u_end, total, programs};
+    }
+  }
+  __syncthreads();
+  return *found;
+}
+
+__device__ __forceinline__ bool next_segment(const ChunkArgs& a, DecodeCursor& k, ChunkSegment& s) {
+  if (k.u >= k.u_end) return false;
+  NewTokens nt = new_tokens(a.cu, a.tokens, k.b);
+  while (k.row >= item_rows(a, nt.count, true)) {  // on to the next request with rows
+    ++k.b;
+    k.row = 0;
+    nt = new_tokens(a.cu, a.tokens, k.b);
+  }
+  const int t0 = k.row * a.tokens_per_item;
+  const int units = item_units(a, nt.count, held_tokens(a.lens, k.b, a.width, a.page), t0);
+  const int count = static_cast<int>(min(static_cast<long long>(units - k.off), k.u_end - k.u));
+  make_segment(a, s, k.b, k.hk, nt, t0, units, k.off, count);
+  s.end_u = k.u - k.off + units;
+  k.u += count;
+  k.off += count;
+  if (k.off >= units) {
+    k.off = 0;
+    if (++k.hk == a.kv_heads) {
+      k.hk = 0;
+      ++k.row;
+    }
+  }
+  return true;
+}
+
 template <typename T, int NB>
 __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
     chunk_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -81,13 +183,17 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], NW);
     }
-    *reinterpret_cast<volatile int*>(smem + S::kFlag + 4) = 0;
+    *reinterpret_cast<volatile int*>(smem + S::kFlag) = 0;
     fence_barrier_init();
   }
-  __syncthreads();
-  grid_dependency_wait();
-  ChunkCursor cur;
-  cursor_init(a, cur);
+  if (threadIdx.x == 0) {
+    a.slots.errors[blockIdx.x] = make_int2(0, 0);
+    a.slots.cuts[blockIdx.x] = {0, 0, 0, -1};
+  }
+  grid_dependents_launch();
+  __shared__ long long scan[S::kThreads / 32];
+  __shared__ DecodeCursor found;
+  DecodeCursor cur = decode_cursor<S::kThreads>(a, scan, &found);
   ChunkSegment sg;
 
   if (warp == NW) {
@@ -113,7 +219,7 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
         const int loads = __popc(__ballot_sync(0xffffffffu, load));
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], phase ^ 1, a.budget_ns));
         if (!ok) {
-          if (lane == 0) record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, 70);
+          if (lane == 0) chunk_error(a, 70);
           break;
         }
         if (lane == 0) mbar_arrive_expect_tx(&full[st], loads * box_bytes);
@@ -135,8 +241,7 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
   float* merge_o = reinterpret_cast<float*>(smem + S::kMergeO);
   float* merge_m = reinterpret_cast<float*>(smem + S::kMergeMl);
   float* merge_l = merge_m + NW * 16;
-  volatile int* merge_flag = reinterpret_cast<volatile int*>(smem + S::kFlag);
-  volatile int* abort_flag = merge_flag + 1;  // a warp's wait gave up: all leave together at the item's first barrier
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kFlag);  // a warp's wait gave up: all leave together at the item's first barrier
   const int g = lane / 4, c2 = (lane % 4) * 2;  // accumulator rows g and g + 8, columns c2 and c2 + 1
   // ldmatrix addresses within a tile: keys of this warp as B of Q K^T (K) and, transposed, of P V (V)
   const int kkey = warp * 16 + (lane / 16) * 8 + lane % 8, kchunk = (lane / 8) % 2;
@@ -174,7 +279,7 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
     for (int j = 0; j < sg.n; ++j) {
       if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, a.budget_ns))) {
         if (lane == 0) {
-          record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, 71);
+          chunk_error(a, 71);
           *abort_flag = 1;
         }
         break;
@@ -306,7 +411,7 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
       }
       named_barrier_sync(1, NW * 32);
     }
-    if (!sg.piece) {
+    if (sg.slot < 0) {
       if (warp == 0) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -323,54 +428,25 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
       }
       continue;
     }
-    // A piece: normalised O and base-2 LSE to its slot, then the piece that completes the set merges all of them in
-    // piece order. No CTA waits for another.
-    const ChunkPieces pieces = chunk_pieces(a, sg);
+    // A piece: normalised O and base-2 LSE to its slot
     if (warp == 0) {
-      const long long slot = pieces.slot(blockIdx.x);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int r = g + 8 * u;
+        const long long at = static_cast<long long>(sg.slot) * kDecodeRows + g + 8 * u;
         const float inv = total[u] > 0.f ? 1.f / total[u] : 0.f;
-        float* out = a.list.slot_o + (slot * kDecodeRows + r) * a.dim;
+        float* out = a.slots.o + at * a.dim;
 #pragma unroll
         for (int i = 0; i < NB * 8; ++i) {
           if (i * 8 < a.dim) *reinterpret_cast<float2*>(out + i * 8 + c2) = make_float2(o[i][2 * u] * inv, o[i][2 * u + 1] * inv);
         }
-        if (lane % 4 == 0) a.list.slot_lse[slot * kDecodeRows + r] = total[u] > 0.f ? top[u] + fast_log2(total[u]) : kEmptyLse;
+        if (lane % 4 == 0) a.slots.lse[at] = total[u] > 0.f ? top[u] + fast_log2(total[u]) : kEmptyLse;
       }
-      __threadfence();
-      __syncwarp();
-      if (lane == 0) *merge_flag = atomicAdd(&a.list.counters[pieces.q_first], 1) + 1 == pieces.pieces ? 1 : 0;
     }
-    named_barrier_sync(1, NW * 32);
-    const bool last = *merge_flag != 0;
-    named_barrier_sync(1, NW * 32);
-    if (!last) continue;
-    __threadfence();
-    const int chunks = a.dim / 4;
-    for (int i = threadIdx.x; i < sg.count * a.group * chunks; i += NW * 32) {
-      const int r = i / chunks, c = i % chunks;
-      float peak = kEmptyLse, sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int p = pieces.q_first; p <= pieces.q_last; ++p) {
-        if (!pieces.holds(p)) continue;
-        const long long at = static_cast<long long>(pieces.slot(p)) * kDecodeRows + r;
-        const float lse = __ldcg(&a.list.slot_lse[at]);
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(a.list.slot_o + at * a.dim) + c);
-        float w_old, w_new;
-        merge_split_weights(lse, peak, sum, w_old, w_new);
-        acc.x = merge_split_accumulate(acc.x, w_old, w_new, x.x);
-        acc.y = merge_split_accumulate(acc.y, w_old, w_new, x.y);
-        acc.z = merge_split_accumulate(acc.z, w_old, w_new, x.z);
-        acc.w = merge_split_accumulate(acc.w, w_old, w_new, x.w);
-      }
-      T* out = static_cast<T*>(a.out) + (sg.token0 + r / a.group) * a.out_stride +
-               static_cast<long long>(sg.hk * a.group + r % a.group) * a.dim + c * 4;
-      *reinterpret_cast<uint2*>(out) = make_uint2(Tr::pack2(merge_split_finish(acc.x, sum), merge_split_finish(acc.y, sum)),
-                                                  Tr::pack2(merge_split_finish(acc.z, sum), merge_split_finish(acc.w, sum)));
+    if (sg.starts && threadIdx.x == 0) {
+      a.slots.cuts[blockIdx.x] = {sg.token0, sg.count, sg.hk, program_of(cur.total, cur.programs, sg.end_u - 1)};
     }
   }
+  grid_dependency_wait();  // so that what follows this kernel follows the plan ahead of it too
 }
 
 template <typename T, int NB>
@@ -383,7 +459,11 @@ static cudaError_t launch_decode_t(const fgw_chunk_params& p, ChunkArgs a, int d
   CUtensorMap kmap, vmap;
   if (chunk_kv_map(&kmap, p, p.k_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
   if (chunk_kv_map(&vmap, p, p.v_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
-  return launch_after_plan(kernel, static_cast<unsigned>(a.programs), S::kThreads, S::kBytes, stream, kmap, vmap, a);
+  if (a.split) {  // the plan of the tensor kernel runs ahead; this kernel does not wait for it
+    return launch_after_plan(kernel, static_cast<unsigned>(a.programs), S::kThreads, S::kBytes, stream, kmap, vmap, a);
+  }
+  kernel<<<a.programs, S::kThreads, S::kBytes, stream>>>(kmap, vmap, a);
+  return cudaGetLastError();
 }
 
 template <typename T>

@@ -42,6 +42,48 @@ struct TensorShape {
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
+// A CTA's whole items, then its range of units of the cut ones.
+struct TensorCursor {
+  int round, rounds, items;
+  int item, off;
+  long long u, u_end;
+};
+
+__device__ __forceinline__ void cursor_init(const ChunkList& list, TensorCursor& k) {
+  k.round = 0;
+  k.rounds = list.meta->rounds;
+  k.items = list.meta->items;
+  k.item = list.prog_item[blockIdx.x];
+  k.off = list.prog_off[blockIdx.x];
+  k.u = list.prog_u[blockIdx.x];
+  k.u_end = list.prog_u[blockIdx.x + 1];
+}
+
+__device__ __forceinline__ bool next_segment(const ChunkArgs& a, const ChunkList& list, TensorCursor& k,
+                                             ChunkSegment& s) {
+  int item = k.items;
+  if (k.round < k.rounds) item = static_cast<int>(snake_item(k.round++));
+  const bool whole = item < k.items;  // the last round may be short
+  if (!whole) {
+    if (k.u >= k.u_end) return false;
+    item = k.item;
+  }
+  const int4 row = list.rows[item / a.kv_heads];
+  const int units = row.z, first = whole ? 0 : k.off;
+  const int count = whole ? units : static_cast<int>(min(static_cast<long long>(units - first), k.u_end - k.u));
+  make_segment(a, s, row.x, item % a.kv_heads, new_tokens(a.cu, a.tokens, row.x), row.y, units, first, count);
+  if (!whole) {
+    s.end_u = k.u - first + units;
+    k.u += count;
+    k.off += count;
+    if (k.off >= units) {
+      ++k.item;
+      k.off = 0;
+    }
+  }
+  return true;
+}
+
 // max(a, b, c) in one instruction (sm_100 three-input max; NaN-free inputs here)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -73,7 +115,8 @@ __device__ __forceinline__ int tile_steps(const ChunkArgs& a, const ChunkSegment
 template <typename T, int NB>
 __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
     chunk_tensor_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ ChunkArgs a) {
+                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ ChunkArgs a,
+                        const __grid_constant__ ChunkList list) {
   using S = TensorShape<NB>;
   using Tr = ElemTraits<T>;
   constexpr int BN = S::kBN, NS = S::kStages, kTiles = S::kTiles;
@@ -96,7 +139,6 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
   uint64_t* o_empty = pv_done + 2;  // [2]
   uint64_t* mma_done = o_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kTmemSlot);
-  volatile int* merge_flag = reinterpret_cast<volatile int*>(smem + S::kTmemSlot + 4);
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
@@ -118,6 +160,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
     }
     mbar_init(mma_done, 1);
     fence_barrier_init();
+    a.slots.errors[blockIdx.x] = make_int2(0, 0);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, S::kTmemCols);
@@ -130,6 +173,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
   const int D = a.dim;
   const int tile_tokens = kTensorTileRows / a.group;
   grid_dependency_wait();  // the plan's lists from here on
+  grid_dependents_launch();
 
   if (kTiles == 2 && warp < 4) setmaxnreg_dec<S::kRegsControl>();
   if (warp == 0) {
@@ -149,14 +193,14 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
     auto wait_or_fail = [&](uint64_t* bar, uint32_t parity, int site) {
       if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity, a.budget_ns))) {
         ok = false;
-        if (lane == 0) record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, site);
+        if (lane == 0) chunk_error(a, site);
       }
       return ok;
     };
-    ChunkCursor cur;
-    cursor_init(a, cur);
+    TensorCursor cur;
+    cursor_init(list, cur);
     ChunkSegment sg;
-    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, cur, sg)), 0)) {
+    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, list, cur, sg)), 0)) {
       const int n = __shfl_sync(0xffffffffu, sg.n, 0);
       if (n <= 0) continue;
       if (wait_or_fail(q_empty, (qc & 1) ^ 1, 80) && lane == 0) {
@@ -211,7 +255,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
     auto wait_or_fail = [&](uint64_t* bar, uint32_t parity, int site) {
       if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity, a.budget_ns))) {
         ok = false;
-        if (lane == 0) record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, site);
+        if (lane == 0) chunk_error(a, site);
       }
       return ok;
     };
@@ -242,10 +286,10 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
         asm volatile("" : "+r"(p_col), "+r"(b_lo));
       }
     };
-    ChunkCursor cur;
-    cursor_init(a, cur);
+    TensorCursor cur;
+    cursor_init(list, cur);
     ChunkSegment sg;
-    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, cur, sg)), 0)) {
+    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, list, cur, sg)), 0)) {
       const int n = __shfl_sync(0xffffffffu, sg.n, 0);
       const int n_a = __shfl_sync(0xffffffffu, tile_steps(a, sg, 0, tile_tokens), 0);
       const int n_b = kTiles == 2 ? __shfl_sync(0xffffffffu, tile_steps(a, sg, 1, tile_tokens), 0) : 0;
@@ -323,17 +367,18 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
     const uint32_t o_addr = tmem + lane_base + S::o_col(t);
     bool ok = true;
     uint32_t sc = 0, pd = 0, vbase = 0;
+    if (warp == 4 && lane == 0) a.slots.cuts[blockIdx.x] = {0, 0, 0, -1};
     auto wait_warp = [&](uint64_t* bar, uint32_t parity, int site) {
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, a.budget_ns));
-        if (!ok && lane == 0) record_error(a.ws, FGW_ERR_DEVICE_TIMEOUT, site);
+        if (!ok && lane == 0) chunk_error(a, site);
       }
       return ok;
     };
-    ChunkCursor cur;
-    cursor_init(a, cur);
+    TensorCursor cur;
+    cursor_init(list, cur);
     ChunkSegment sg;
-    while (next_segment(a, cur, sg)) {
+    while (next_segment(a, list, cur, sg)) {
       const int i_tok = t * tile_tokens + row_token;  // token within the item
       const bool row_valid = row_token < tile_tokens && i_tok < sg.count;
       // rows of no token compute on whatever Q's tile holds (rows do not mix) and are never stored
@@ -467,18 +512,16 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
           for (int i = 0; i < 16; ++i) o[i] = 0.f;
         }
       };
-      auto store_row = [&](int cb, const float (&o)[16], float scale) {
-        uint4* dst = reinterpret_cast<uint4*>(out_row + cb * 16);
-        dst[0] = make_uint4(Tr::pack2(o[0] * scale, o[1] * scale), Tr::pack2(o[2] * scale, o[3] * scale),
-                            Tr::pack2(o[4] * scale, o[5] * scale), Tr::pack2(o[6] * scale, o[7] * scale));
-        dst[1] = make_uint4(Tr::pack2(o[8] * scale, o[9] * scale), Tr::pack2(o[10] * scale, o[11] * scale),
-                            Tr::pack2(o[12] * scale, o[13] * scale), Tr::pack2(o[14] * scale, o[15] * scale));
-      };
-      if (!sg.piece) {
+      if (sg.slot < 0) {
         for (int cb = 0; cb < D / 16; ++cb) {
           float o[16];
           load_o(cb, o);  // warp-collective: every lane, valid row or not
-          if (row_valid) store_row(cb, o, 1.f);
+          if (row_valid) {
+            uint4* dst = reinterpret_cast<uint4*>(out_row + cb * 16);
+            dst[0] = make_uint4(Tr::pack2(o[0], o[1]), Tr::pack2(o[2], o[3]), Tr::pack2(o[4], o[5]), Tr::pack2(o[6], o[7]));
+            dst[1] = make_uint4(Tr::pack2(o[8], o[9]), Tr::pack2(o[10], o[11]), Tr::pack2(o[12], o[13]),
+                                Tr::pack2(o[14], o[15]));
+          }
         }
         if (n_t > 0) {
           tc_fence_before_sync();
@@ -487,89 +530,33 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
         }
         continue;
       }
-      // A piece of an item cut between CTAs: FP32 O and base-2 LSE go to its slot (O in groups of four columns,
-      // [D / 4][rows][4], so a warp's rows write 512 contiguous bytes per group), and the piece that completes the set
-      // merges all pieces in their order. No CTA waits for another.
+      // A piece of an item cut between CTAs: FP32 O and base-2 LSE go to its slot, O in groups of four columns ([D / 4]
+      // [rows][4]), so a warp's rows write 512 contiguous bytes per group.
       constexpr int kSlotRows = kTensorTileRows * kTiles;
       const int r = kTensorTileRows * t + row;
-      auto slot_group = [&](int slot, int g) -> float4* {
-        return reinterpret_cast<float4*>(a.list.slot_o) + (static_cast<long long>(slot) * (D / 4) + g) * kSlotRows + r;
-      };
-      const ChunkPieces pieces = chunk_pieces(a, sg);
-      const int my_slot = pieces.slot(blockIdx.x);
+      float4* slot_o = reinterpret_cast<float4*>(a.slots.o) + static_cast<long long>(sg.slot) * (D / 4) * kSlotRows + r;
       for (int cb = 0; cb < D / 16; ++cb) {
         float o[16];
         load_o(cb, o);
         if (row_valid) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            *slot_group(my_slot, cb * 4 + i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            slot_o[(cb * 4 + i) * kSlotRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
       }
       if (row_valid) {
-        a.list.slot_lse[static_cast<long long>(my_slot) * kSlotRows + r] =
-            (n_t > 0 && l > 0.f) ? m + fast_log2(l) : kEmptyLse;
+        a.slots.lse[static_cast<long long>(sg.slot) * kSlotRows + r] = (n_t > 0 && l > 0.f) ? m + fast_log2(l) : kEmptyLse;
       }
       if (n_t > 0) {
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&o_empty[t]);
       }
-      named_barrier_sync(1, 128 * kTiles);
-      if (warp == 4 && lane == 0) {
-        __threadfence();
-        *merge_flag = atomicAdd(&a.list.counters[pieces.q_first], 1) + 1 == pieces.pieces ? 1 : 0;
-      }
-      named_barrier_sync(1, 128 * kTiles);
-      const int merge = *merge_flag;
-      named_barrier_sync(1, 128 * kTiles);  // read by all before the next write
-      if (merge == 0) continue;
-      __threadfence();
-      if (!row_valid) continue;
-      auto lse_of = [&](int p) { return __ldcg(&a.list.slot_lse[static_cast<long long>(pieces.slot(p)) * kSlotRows + r]); };
-      float peak = kEmptyLse, wsum = 0.f;
-      for (int p = pieces.q_first; p <= pieces.q_last; ++p) {
-        if (pieces.holds(p)) peak = fmaxf(peak, lse_of(p));
-      }
-      auto weight = [&](int p) {
-        const float lse = lse_of(p);
-        return lse > kValidLse ? fast_exp2(lse - peak) : 0.f;
-      };
-      for (int p = pieces.q_first; p <= pieces.q_last; ++p) {
-        if (pieces.holds(p)) wsum += weight(p);
-      }
-      const float scale = wsum > 0.f ? 1.f / wsum : 0.f;
-      // 32 values of every piece per round with independent 16-byte loads
-      for (int cb = 0; cb < D / 16; cb += 2) {
-        const bool second = cb + 1 < D / 16;
-        float acc0[16], acc1[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc0[i] = acc1[i] = 0.f;
-        for (int p = pieces.q_first; p <= pieces.q_last; ++p) {
-          if (!pieces.holds(p)) continue;
-          const float wk = weight(p);
-          if (wk == 0.f) continue;
-          const int slot = pieces.slot(p);
-          float4 v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = (i < 4 || second) ? __ldcg(slot_group(slot, cb * 4 + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            acc0[4 * i] = fmaf(wk, v[i].x, acc0[4 * i]);
-            acc0[4 * i + 1] = fmaf(wk, v[i].y, acc0[4 * i + 1]);
-            acc0[4 * i + 2] = fmaf(wk, v[i].z, acc0[4 * i + 2]);
-            acc0[4 * i + 3] = fmaf(wk, v[i].w, acc0[4 * i + 3]);
-            acc1[4 * i] = fmaf(wk, v[4 + i].x, acc1[4 * i]);
-            acc1[4 * i + 1] = fmaf(wk, v[4 + i].y, acc1[4 * i + 1]);
-            acc1[4 * i + 2] = fmaf(wk, v[4 + i].z, acc1[4 * i + 2]);
-            acc1[4 * i + 3] = fmaf(wk, v[4 + i].w, acc1[4 * i + 3]);
-          }
-        }
-        store_row(cb, acc0, scale);
-        if (second) store_row(cb + 1, acc1, scale);
+      if (sg.starts && warp == 4 && lane == 0) {
+        int last = blockIdx.x;
+        while (list.prog_u[last + 1] < sg.end_u) ++last;
+        a.slots.cuts[blockIdx.x] = {sg.token0, sg.count, sg.hk, last};
       }
     }
   }
@@ -582,7 +569,8 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
 }
 
 template <typename T, int NB>
-static cudaError_t launch_tensor_t(const fgw_chunk_params& p, ChunkArgs a, int device, cudaStream_t stream) {
+static cudaError_t launch_tensor_t(const fgw_chunk_params& p, ChunkArgs a, const ChunkList& list, int device,
+                                   cudaStream_t stream) {
   using S = TensorShape<NB>;
   auto kernel = chunk_tensor_kernel<T, NB>;
   int regs = 0;
@@ -612,26 +600,28 @@ static cudaError_t launch_tensor_t(const fgw_chunk_params& p, ChunkArgs a, int d
   if (chunk_kv_map(&kmap, p, p.k_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
   if (chunk_kv_map(&vmap, p, p.v_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
   return launch_after_plan(kernel, static_cast<unsigned>(a.programs), S::kThreads, S::kBytes, stream, qmap, kmap, vmap,
-                           a);
+                           a, list);
 }
 
 template <typename T>
-static cudaError_t launch_tensor_nb(const fgw_chunk_params& p, const ChunkArgs& a, int device, cudaStream_t stream) {
+static cudaError_t launch_tensor_nb(const fgw_chunk_params& p, const ChunkArgs& a, const ChunkList& list, int device,
+                                    cudaStream_t stream) {
   switch ((p.head_dim + 63) / 64) {
     case 1:
-      return launch_tensor_t<T, 1>(p, a, device, stream);
+      return launch_tensor_t<T, 1>(p, a, list, device, stream);
     case 2:
-      return launch_tensor_t<T, 2>(p, a, device, stream);
+      return launch_tensor_t<T, 2>(p, a, list, device, stream);
     case 3:
-      return launch_tensor_t<T, 3>(p, a, device, stream);
+      return launch_tensor_t<T, 3>(p, a, list, device, stream);
     default:
-      return launch_tensor_t<T, 4>(p, a, device, stream);
+      return launch_tensor_t<T, 4>(p, a, list, device, stream);
   }
 }
 
-cudaError_t launch_chunk_tensor(const fgw_chunk_params& p, ChunkArgs a, int device, cudaStream_t stream) {
-  return p.dtype == FGW_DTYPE_BFLOAT16 ? launch_tensor_nb<__nv_bfloat16>(p, a, device, stream)
-                                       : launch_tensor_nb<__half>(p, a, device, stream);
+cudaError_t launch_chunk_tensor(const fgw_chunk_params& p, ChunkArgs a, const ChunkList& list, int device,
+                                   cudaStream_t stream) {
+  return p.dtype == FGW_DTYPE_BFLOAT16 ? launch_tensor_nb<__nv_bfloat16>(p, a, list, device, stream)
+                                       : launch_tensor_nb<__half>(p, a, list, device, stream);
 }
 
 }  // namespace fgw
