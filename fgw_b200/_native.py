@@ -5,6 +5,7 @@ There is no fallback: if the library is missing or cannot be loaded, every entry
 ``NativeLibraryError`` naming the file, so a GPU box without the built extension fails loudly.
 """
 import ctypes
+import functools
 import pathlib
 
 import numpy as np
@@ -210,6 +211,20 @@ class PageParams(ctypes.Structure):
     _fields_ += [("reserved", ctypes.c_int32 * 2)]
 
 
+_FORMATS = {ctypes.c_void_p: "Q", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f",
+            ctypes.c_int32 * 2: "2i"}
+
+
+def struct_format(cls):
+    """``struct`` format of a parameter structure, for callers that pack it as bytes in one call."""
+    return "@" + "".join(_FORMATS[kind] for _, kind in cls._fields_)
+
+
+def address_of(data):
+    """Address of a bytes object's contents (valid while the caller holds it)."""
+    return ctypes.cast(data, ctypes.c_void_p).value
+
+
 _LIB = None
 
 
@@ -393,9 +408,12 @@ def paged_cache_gather(params, stream_ptr):
           "fgw_paged_cache_gather")
 
 
+# The params of the calls below are the parameter structure packed as bytes.
 def rotary_append(params, stream_ptr):
     """``fgw_rotary_append``: rotate the new tokens' queries and keys and append keys and values to the cache."""
-    check(library().fgw_rotary_append(ctypes.byref(params), stream_ptr), "fgw_rotary_append")
+    status = library().fgw_rotary_append(params, stream_ptr)
+    if status:
+        raise FgwError(status, "fgw_rotary_append")
 
 
 def chunk_workspace_size(params):
@@ -406,24 +424,28 @@ def chunk_workspace_size(params):
 
 def chunk_attention(params, workspace_ptr, workspace_bytes, stream_ptr):
     """``fgw_chunk_attention``: attention of the new tokens over the cache."""
-    check(library().fgw_chunk_attention(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr),
-          "fgw_chunk_attention")
+    status = library().fgw_chunk_attention(params, workspace_ptr, workspace_bytes, stream_ptr)
+    if status:
+        raise FgwError(status, "fgw_chunk_attention")
 
 
-def page_workspace_size(params):
+@functools.lru_cache(maxsize=256)
+def page_workspace_bytes(batch, num_pages, copy_count):
+    """``fgw_page_workspace_size`` of a fork or compaction of ``batch`` rows, or (batch 0) of a list of copies."""
+    p = PageParams()
+    p.batch, p.num_pages, p.copy_count = batch, num_pages, copy_count
     out = ctypes.c_size_t(0)
-    check(library().fgw_page_workspace_size(ctypes.byref(params), ctypes.byref(out)), "fgw_page_workspace_size")
+    check(library().fgw_page_workspace_size(ctypes.byref(p), ctypes.byref(out)), "fgw_page_workspace_size")
     return out.value
 
 
 def page_fork(params, workspace_ptr, workspace_bytes, stream_ptr):
-    check(library().fgw_page_fork(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_fork")
+    check(library().fgw_page_fork(params, workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_fork")
 
 
 def page_compact(params, workspace_ptr, workspace_bytes, stream_ptr):
-    check(library().fgw_page_compact(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr),
-          "fgw_page_compact")
+    check(library().fgw_page_compact(params, workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_compact")
 
 
 def page_copy(params, workspace_ptr, workspace_bytes, stream_ptr):
-    check(library().fgw_page_copy(ctypes.byref(params), workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_copy")
+    check(library().fgw_page_copy(params, workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_copy")

@@ -4,10 +4,10 @@
 // out[t, h] = sum_j softmax_j(scale q[t, h] . k[j, h / G]) v[j, h / G] over the first vis(t) cached tokens of t's request:
 // vis = len - n + i + 1 for the i-th of its n new tokens when causal, len otherwise; rows with vis <= 0 are zeros.
 //
-// Two kernels share the work, each request going whole to one of them: requests with at most 16 (token, head of a group)
-// rows per key head to the decode kernel (fgw_chunk_decode.cu, bound by HBM), the others to the tensor kernel
-// (fgw_chunk_sm100.cu, tcgen05). Lengths are device data, so the host does not know which requests are which: with at
-// most 16 rows per request on average it launches the decode kernel alone, which then takes everything (a longer
+// Two kernels share the work, each request going whole to one of them: requests with few (token, head of a group) rows per
+// key head to the decode kernel (fgw_chunk_decode.cu, bound by HBM), the others to the tensor kernel
+// (fgw_chunk_sm100.cu, tcgen05). Lengths are device data, so the host does not know which requests are which: when the
+// requests' average rows fit an item of the decode kernel it launches that alone, which then takes everything (a longer
 // request in several items), else both. The plan (tensor kernel only), decode, tensor and merge kernels follow one
 // another as programmatic dependent launches, so each one's set-up overlaps the one before.
 #include <algorithm>
@@ -373,9 +373,17 @@ CUresult chunk_kv_map(CUtensorMap* map, const fgw_chunk_params& p, const void* b
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
-static bool decode_on(const fgw_chunk_params& p) { return p.heads / p.kv_heads <= kDecodeRows; }
+// Rows of a decode item (16, 32 or, up to D = 128, 64): enough for the requests' average rows where that is at all
+// possible, else (chunks among them) for single tokens, which are then its work.
+static int decode_rows(const fgw_chunk_params& p) {
+  const long long group = p.heads / p.kv_heads, most = p.head_dim <= 128 ? 64 : 32;
+  const long long average = (p.tokens * group + p.batch - 1) / p.batch;
+  const long long want = std::max(average <= most ? average : 0, group);
+  return want <= 16 ? 16 : static_cast<int>(std::min<long long>(most, want <= 32 ? 32 : 64));
+}
+static bool decode_on(const fgw_chunk_params& p) { return p.heads / p.kv_heads <= decode_rows(p); }
 static bool tensor_on(const fgw_chunk_params& p) {
-  return !decode_on(p) || p.tokens * (p.heads / p.kv_heads) > static_cast<long long>(kDecodeRows) * p.batch;
+  return !decode_on(p) || p.tokens * (p.heads / p.kv_heads) > static_cast<long long>(decode_rows(p)) * p.batch;
 }
 
 // The workspace from `at` on (sizes alone when it is null), by class: slots of both kernels, the tensor kernel's list.
@@ -398,9 +406,9 @@ static ChunkLayout chunk_layout(const fgw_chunk_params& p, uint8_t* const begin)
   take(sizeof(WorkspaceHeader));
   const size_t programs = kStreamMaxPrograms;
   const bool on[2] = {decode_on(p), tensor_on(p)};
-  l.tokens_per_item[0] = kDecodeRows / group;
-  l.keys_per_unit[0] = chunk_decode_keys(nb);
-  l.slot_rows[0] = kDecodeRows;
+  l.tokens_per_item[0] = decode_rows(p) / group;
+  l.keys_per_unit[0] = chunk_decode_keys(nb, decode_rows(p) / 16);
+  l.slot_rows[0] = decode_rows(p);
   l.tokens_per_item[1] = kTensorTileRows / group * chunk_tensor_tiles(nb);
   l.keys_per_unit[1] = 128;
   l.slot_rows[1] = kTensorTileRows * chunk_tensor_tiles(nb);
@@ -451,6 +459,7 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_coun
   a[0].page = p.page_size;
   a[0].causal = p.causal;
   a[0].programs = std::min(sm_count, kStreamMaxPrograms);
+  a[0].small_rows = decode_rows(p);
   a[0].split = on[0] && on[1] ? 1 : 0;
   a[0].scale_log2 = p.softmax_scale * kLog2e;
   a[0].budget_ns = static_cast<uint64_t>(p.wait_budget_ms > 0 ? p.wait_budget_ms : 2000) * 1000000ull;

@@ -15,7 +15,6 @@
 
 namespace fgw {
 
-constexpr int kDecodeRows = 16;      // rows of a decode item: one m16 MMA tile
 constexpr int kTensorTileRows = 128;
 
 // The item whose first piece a program holds when that item goes on in later programs; last < 0: none.
@@ -58,7 +57,8 @@ struct ChunkArgs {
   long long tokens, q_stride, out_stride;
   int batch, heads, kv_heads, group, dim, width, page, causal, box_rows, programs;
   int tokens_per_item, keys_per_unit;
-  int split;  // requests go by their rows; otherwise everything is the launched kernel's
+  int small_rows;  // rows of a decode item; requests of at most so many go to the decode kernel
+  int split;       // requests go by their rows; otherwise everything is the launched kernel's
   float scale_log2;
   uint64_t budget_ns;
   ChunkSlots slots;
@@ -85,7 +85,7 @@ __device__ __forceinline__ int held_tokens(const int32_t* lens, int b, int width
 
 // Rows of the request's list, 0 when it belongs to the other kernel.
 __device__ __forceinline__ int item_rows(const ChunkArgs& a, int count, bool decode) {
-  if (a.split && (count * a.group <= kDecodeRows) != decode) return 0;
+  if (a.split && (count * a.group <= a.small_rows) != decode) return 0;
   return (count + a.tokens_per_item - 1) / a.tokens_per_item;
 }
 
@@ -142,7 +142,7 @@ CUresult chunk_kv_map(CUtensorMap* map, const fgw_chunk_params& p, const void* b
 int chunk_box_rows(int page, int keys);
 
 // Per-width shapes of the two kernels (D up to 64, 128, 192, 256: NB = 1..4 blocks of 64 values).
-__host__ __device__ constexpr int chunk_decode_keys(int nb) { return nb <= 2 ? 128 : 64; }
+__host__ __device__ constexpr int chunk_decode_keys(int nb, int row_tiles) { return nb <= 2 && row_tiles <= 2 ? 128 : 64; }
 __host__ __device__ constexpr int chunk_tensor_tiles(int nb) { return nb <= 2 ? 2 : 1; }
 
 }  // namespace fgw

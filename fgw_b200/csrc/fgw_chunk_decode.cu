@@ -1,13 +1,15 @@
-// Chunk attention, decode kernel: items of at most 16 (token, query head) rows of one request and key head.
+// Chunk attention, decode kernel: items of at most 16, 32 or 64 (token, query head) rows of one request and key
+// head.
 //
-// Bound by HBM: each item reads its K and V once and computes 2 x 16 x D products per key, so the kernel is a stream of
-// K/V tiles with little arithmetic behind it. One persistent CTA per SM: a producer warp keeps a ring of K/V tiles full
-// (TMA through the page table, 192 KB in flight or in use), and each consumer warp owns 16 keys of every tile, which it
-// carries alone from scores to weighted values: S = Q K^T and O += P V with m16n8k16 MMAs on the 16 rows, its own running
-// maximum and sum, P kept in registers (the score accumulator's layout is the A operand's). So no warp waits for
-// another until the item ends, where the warps' states are merged in a fixed order through shared memory. The tensor
-// units of a tile this small would sit idle in tcgen05's 128-row form: 16 rows leave seven eighths of it empty, and
-// its scores would cross TMEM twice.
+// Bound by HBM: each item reads its K and V once and computes little per byte, so the kernel is a stream of K/V tiles
+// with a short chain of arithmetic behind it. One persistent CTA per SM: a producer warp keeps a ring of K/V tiles full
+// (TMA through the page table, about 190 KB in flight or in use), eight consumer warps share each tile: scores by keys
+// (a warp takes 16 or 8 of them), one exchange of row maxima through shared memory, P to shared memory, then P V by
+// values (a warp takes an eighth of the head). So a warp holds an eighth of O, nothing is left to add up across warps
+// at the end of an item, and up to 64 rows fit; two barriers of the eight warps per tile are the price. (Each warp
+// carrying its own keys to the end, with the whole O of 16 rows in registers, needed no barrier per tile but took 5200
+// cycles to merge the warps' states: 25.0 us against XXX us for eight single tokens.) m16n8k16 MMAs: tcgen05's
+// 128-row form would leave most rows of its tile empty and carry the scores through TMEM twice.
 //
 // The work is split without a plan kernel: every CTA sums the units of all requests and finds the start of its own
 // range. That costs two or three trips to L2 before the first load; a plan launch ahead of it measured 6 us more.
@@ -22,21 +24,29 @@ namespace fgw {
 
 constexpr int kDecodeMinUnits = 2;  // units a program takes at least: a piece costs a merge
 
-template <int NB>
+// NB blocks of 64 values per head, MT tiles of 16 rows per item.
+template <int NB, int MT>
 struct DecodeShape {
-  static constexpr int kBN = chunk_decode_keys(NB);
-  static constexpr int kWarps = kBN / 16;              // consumer warps
+  static constexpr int kBN = chunk_decode_keys(NB, MT);
+  static constexpr int kWarps = 8;                     // consumer warps
   static constexpr int kThreads = 32 * (kWarps + 1);
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kDim = NB * 64;
+  static constexpr int kKeys = kBN / kWarps;           // keys of a warp: 16 or 8
   static constexpr int kBlockBytes = kBN * 128;        // 64 values of every key
   static constexpr int kTileBytes = NB * kBlockBytes;  // K or V tile
-  static constexpr int kStages = (192 * 1024) / (2 * kTileBytes);
-  static constexpr int kDim = NB * 64;
-  static constexpr int kMergeO = kStages * 2 * kTileBytes;                  // [kWarps / 2][16][kDim] floats
-  static constexpr int kMergeMl = kMergeO + kWarps / 2 * 16 * kDim * 4;     // [kWarps][16] maxima, then sums
-  static constexpr int kBar = kMergeMl + 2 * kWarps * 16 * 4;
+  static constexpr int kQBytes = kRows * kDim * 2;
+  static constexpr int kPBytes = kRows * kBN * 2;
+  static constexpr int kMaxBytes = kRows * kWarps * 4;
+  static constexpr int kRoom = 232448 - 2048 - kQBytes - kPBytes - kMaxBytes;
+  static constexpr int kStages = kRoom / (2 * kTileBytes) < 8 ? kRoom / (2 * kTileBytes) : 8;
+  static constexpr int kQ = kStages * 2 * kTileBytes;
+  static constexpr int kP = kQ + kQBytes;
+  static constexpr int kMax = kP + kPBytes;            // [kRows][kWarps] maxima, then sums
+  static constexpr int kBar = kMax + kMaxBytes;
   static constexpr int kFlag = kBar + 2 * kStages * 8;
   static constexpr int kBytes = kFlag + 16 + 1024;
-  static_assert(kBytes <= 232448, "shared memory of one CTA");
+  static_assert(kBytes + 512 <= 232448 && kStages >= 2, "shared memory of one CTA");
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
@@ -166,48 +176,50 @@ __device__ __forceinline__ bool next_segment(const ChunkArgs& a, DecodeCursor& k
   return true;
 }
 
-template <typename T, int NB>
-__global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile of 128-byte rows, blocks of 64 values `block` bytes apart,
+// in TMA's 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk, int block) {
+  return (chunk >> 3) * block + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+template <typename T, int NB, int MT>
+__global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
     chunk_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const __grid_constant__ ChunkArgs a) {
-  using S = DecodeShape<NB>;
+  using S = DecodeShape<NB, MT>;
   using Tr = ElemTraits<T>;
-  constexpr int NS = S::kStages, NW = S::kWarps, BN = S::kBN;
+  constexpr int NS = S::kStages, NW = S::kWarps, BN = S::kBN, kRows = S::kRows;
+  constexpr int kConsumers = NW * 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar);
   uint64_t* empty = full + NS;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kFlag);  // a consumer's wait gave up
+  __shared__ long long scan[S::kThreads / 32];
+  __shared__ DecodeCursor found;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], NW);
     }
-    *reinterpret_cast<volatile int*>(smem + S::kFlag) = 0;
+    *abort_flag = 0;
     fence_barrier_init();
-  }
-  if (threadIdx.x == 0) {
     a.slots.errors[blockIdx.x] = make_int2(0, 0);
     a.slots.cuts[blockIdx.x] = {0, 0, 0, -1};
   }
   grid_dependents_launch();
-  __shared__ long long scan[S::kThreads / 32];
-  __shared__ DecodeCursor found;
-  DecodeCursor cur = decode_cursor<S::kThreads>(a, scan, &found);
+  DecodeCursor cur = decode_cursor<S::kThreads>(a, scan, &found);  // with barriers of the whole CTA
   ChunkSegment sg;
 
   if (warp == NW) {
     // ---------------------------------------------------------------------------------- producer
     // Lane l issues the l-th box of a tile: boxes x blocks of 64 values x {K, V}, at most 32 of them.
     const int boxes = BN / a.box_rows;
-    const int which = lane / (boxes * NB);         // 0: K, 1: V, more: idle
+    const int which = lane / (boxes * NB);  // 0: K, 1: V, more: idle
     const int box = lane % boxes, blk = (lane / boxes) % NB;
     const uint32_t box_bytes = a.box_rows * 128;
     const uint64_t policy = l2_policy_evict_first();
-    if (lane == 0) {
-      tma_prefetch_desc(&kmap);
-      tma_prefetch_desc(&vmap);
-    }
     bool ok = true;
     uint32_t st = 0, phase = 0;
     while (ok && next_segment(a, cur, sg)) {
@@ -238,117 +250,175 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
   }
 
   // ------------------------------------------------------------------------------------ consumers
-  float* merge_o = reinterpret_cast<float*>(smem + S::kMergeO);
-  float* merge_m = reinterpret_cast<float*>(smem + S::kMergeMl);
-  float* merge_l = merge_m + NW * 16;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kFlag);  // a warp's wait gave up: all leave together at the item's first barrier
+  float* row_max = reinterpret_cast<float*>(smem + S::kMax);  // [row][warp]
   const int g = lane / 4, c2 = (lane % 4) * 2;  // accumulator rows g and g + 8, columns c2 and c2 + 1
-  // ldmatrix addresses within a tile: keys of this warp as B of Q K^T (K) and, transposed, of P V (V)
-  const int kkey = warp * 16 + (lane / 16) * 8 + lane % 8, kchunk = (lane / 8) % 2;
-  const int vkey = warp * 16 + (lane / 8) % 2 * 8 + lane % 8, vchunk = lane / 16;
   const uint32_t base = smem_u32(smem);
+  const uint32_t q_at = base + S::kQ, p_at = base + S::kP;
   uint32_t st = 0, phase = 0;
   while (next_segment(a, cur, sg)) {
-    // Q of the item's rows as A operands, straight from global memory
-    uint32_t q[NB * 4][4];
-    int seen[2];
-    long long row_q[2], row_o[2];
+    int seen[MT][2];
+    long long out_at[MT][2];  // element offset of the row's output, -1: no row
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = g + 8 * u, i = r / a.group;
-      const bool valid = i < sg.count;
-      seen[u] = valid ? seen_keys(a, sg, i) : 0;
-      const long long head = static_cast<long long>(sg.hk * a.group + r % a.group) * a.dim;
-      row_q[u] = valid ? (sg.token0 + i) * a.q_stride + head : -1;
-      row_o[u] = valid ? (sg.token0 + i) * a.out_stride + head : -1;
-    }
+    for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-    for (int ks = 0; ks < NB * 4; ++ks) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {  // rows g, g + 8, then the same rows eight values on
-        const int at = ks * 16 + (u / 2) * 8 + c2;
-        q[ks][u] = row_q[u % 2] >= 0 && at < a.dim
-                       ? __ldg(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + row_q[u % 2] + at))
-                       : 0u;
+      for (int u = 0; u < 2; ++u) {
+        const int r = mt * 16 + g + 8 * u, i = r / a.group;
+        const bool valid = i < sg.count;
+        seen[mt][u] = valid ? seen_keys(a, sg, i) : 0;
+        out_at[mt][u] = valid ? (sg.token0 + i) * a.out_stride + static_cast<long long>(sg.hk * a.group + r % a.group) * a.dim
+                              : -1;
       }
     }
-    float o[NB * 8][4];
+    if (sg.n == 0) {  // no keys: zeros
+      for (int i = threadIdx.x; i < sg.count * a.group * a.dim / 8; i += kConsumers) {
+        const int r = i / (a.dim / 8);
+        T* out = static_cast<T*>(a.out) + (sg.token0 + r / a.group) * a.out_stride +
+                 static_cast<long long>(sg.hk * a.group + r % a.group) * a.dim;
+        reinterpret_cast<uint4*>(out)[i % (a.dim / 8)] = make_uint4(0, 0, 0, 0);
+      }
+      continue;
+    }
+    // Q of the item's rows to shared memory
+    for (int i = threadIdx.x; i < kRows * S::kDim / 8; i += kConsumers) {
+      const int r = i / (S::kDim / 8), chunk = i % (S::kDim / 8);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < sg.count * a.group && chunk * 8 < a.dim) {
+        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (sg.token0 + r / a.group) * a.q_stride +
+                                                 static_cast<long long>(sg.hk * a.group + r % a.group) * a.dim) + chunk);
+      }
+      *reinterpret_cast<uint4*>(smem + S::kQ + swizzled(r, chunk, kRows * 128)) = x;
+    }
+    named_barrier_sync(1, kConsumers);
+    float o[MT][NB][4], m[MT][2], l[MT][2];
 #pragma unroll
-    for (int i = 0; i < NB * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+    }
     for (int j = 0; j < sg.n; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, a.budget_ns))) {
-        if (lane == 0) {
-          chunk_error(a, 71);
-          *abort_flag = 1;
-        }
-        break;
+      const bool got = __all_sync(0xffffffffu, mbar_wait(&full[st], phase, a.budget_ns));
+      if (!got && lane == 0) {
+        chunk_error(a, 71);
+        *abort_flag = 1;
       }
-      const int key0 = (sg.n_begin + j) * BN + warp * 16;  // this warp's first key
+      const int key0 = (sg.n_begin + j) * BN + warp * S::kKeys;  // this warp's first key
       const uint32_t ktile = base + 2 * st * S::kTileBytes, vtile = ktile + S::kTileBytes;
-      if (key0 < sg.limit) {
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      constexpr int NT = S::kKeys / 8;
+      float s[MT][NT][4];
 #pragma unroll
-        for (int ks = 0; ks < NB * 4; ++ks) {
-          const int chunk = (ks % 4) * 2 + kchunk;
-          uint32_t b[4];
-          ldmatrix_x4(b, ktile + (ks / 4) * S::kBlockBytes + kkey * 128 + ((chunk ^ (kkey % 8)) * 16));
-          mma_16816<T>(s[0], q[ks], b[0], b[1]);
-          mma_16816<T>(s[1], q[ks], b[2], b[3]);
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) s[mt][i][0] = s[mt][i][1] = s[mt][i][2] = s[mt][i][3] = 0.f;
+      }
+      // S = Q K^T, 16 values per step; with 8 keys one ldmatrix serves two steps
+#pragma unroll
+      for (int ks = 0; ks < NB * 4; ks += 3 - NT) {
+        uint32_t b[4];
+        if constexpr (NT == 2) {
+          ldmatrix_x4(b, ktile + swizzled(warp * 16 + (lane / 16) * 8 + lane % 8, ks * 2 + (lane / 8) % 2, S::kBlockBytes));
+        } else {
+          ldmatrix_x4(b, ktile + swizzled(warp * 8 + lane % 8, ks * 2 + lane / 8, S::kBlockBytes));
         }
-        if (key0 + 16 > sg.limit) {
-          // V rows past the last visible key
-          if (lane < 16 && key0 + lane >= sg.limit) {
-            uint8_t* row = smem + (2 * st + 1) * S::kTileBytes + (warp * 16 + lane) * 128;
 #pragma unroll
-            for (int blk = 0; blk < NB; ++blk) {
+        for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-              for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(row + blk * S::kBlockBytes + c * 16) = make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < 3 - NT; ++k) {
+            uint32_t q[4];
+            ldmatrix_x4(q, q_at + swizzled(mt * 16 + lane % 16, (ks + k) * 2 + lane / 16, kRows * 128));
+            if constexpr (NT == 2) {
+              mma_16816<T>(s[mt][0], q, b[0], b[1]);
+              mma_16816<T>(s[mt][NT - 1], q, b[2], b[3]);
+            } else {
+              mma_16816<T>(s[mt][0], q, b[2 * k], b[2 * k + 1]);
             }
           }
-          fence_proxy_async_smem();  // the ring's next TMA write to these rows comes after
-          __syncwarp();
         }
-        uint32_t p[4];
+      }
+      // keys a row does not see, then the warp's part of the row maxima
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {  // rows g and g + 8
-          float x[4] = {s[0][2 * u], s[0][2 * u + 1], s[1][2 * u], s[1][2 * u + 1]};
-          if (key0 + 16 > seen[u]) {
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (key0 + (i / 2) * 8 + c2 + i % 2 >= seen[u]) x[i] = -INFINITY;
+        for (int u = 0; u < 2; ++u) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = s[mt][i][2 * u + e];
+              if (key0 + i * 8 + c2 + e >= seen[mt][u]) x = -INFINITY;
+              top = fmaxf(top, x);
             }
           }
-          float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float next = fmaxf(m[u], top * a.scale_log2);
-          const float ref = next == -INFINITY ? 0.f : next;
-          if (__any_sync(0xffffffffu, next > m[u])) {
-            const float keep = fast_exp2(m[u] - ref);
-            l[u] *= keep;
+          if (lane % 4 == 0) row_max[(mt * 16 + g + 8 * u) * NW + warp] = top;
+        }
+      }
+      if (key0 + S::kKeys > sg.limit) {
+        // V rows past the last visible key hold whatever the ring or the page holds, and a zero weight times NaN is NaN
+        if (lane < S::kKeys && key0 + lane >= sg.limit) {
+          uint8_t* row = smem + (2 * st + 1) * S::kTileBytes + (warp * S::kKeys + lane) * 128;
 #pragma unroll
-            for (int i = 0; i < NB * 8; ++i) {
-              o[i][2 * u] *= keep;
-              o[i][2 * u + 1] *= keep;
-            }
+          for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(row + blk * S::kBlockBytes + c * 16) = make_uint4(0, 0, 0, 0);
           }
-          m[u] = next;
+        }
+        fence_proxy_async_smem();  // the ring's next TMA write to these rows comes after
+      }
+      named_barrier_sync(1, kConsumers);
+      if (*abort_flag != 0) return;  // all warps read it here, between the same two barriers
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = fast_exp2(fmaf(x[i], a.scale_log2, -ref));
-          p[u] = Tr::pack2(x[0], x[1]);
-          p[2 + u] = Tr::pack2(x[2], x[3]);
-          // the sum is over the rounded weights that multiply V
-          const float2 lo = Tr::unpack2(p[u]), hi = Tr::unpack2(p[2 + u]);
-          l[u] += (lo.x + lo.y) + (hi.x + hi.y);
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = mt * 16 + g + 8 * u;
+          const float4 t0 = *reinterpret_cast<const float4*>(&row_max[r * NW]);
+          const float4 t1 = *reinterpret_cast<const float4*>(&row_max[r * NW + 4]);
+          const float top = fmaxf(fmaxf(fmaxf(t0.x, t0.y), fmaxf(t0.z, t0.w)), fmaxf(fmaxf(t1.x, t1.y), fmaxf(t1.z, t1.w)));
+          const float next = fmaxf(m[mt][u], top * a.scale_log2);  // scale > 0; -inf stays -inf
+          const float ref = next == -INFINITY ? 0.f : next;
+          const float keep = fast_exp2(m[mt][u] - ref);
+          l[mt][u] *= keep;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            o[mt][i][2 * u] *= keep;
+            o[mt][i][2 * u + 1] *= keep;
+          }
+          m[mt][u] = next;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const uint32_t p = Tr::pack2(fast_exp2(fmaf(s[mt][i][2 * u], a.scale_log2, -ref)),
+                                         fast_exp2(fmaf(s[mt][i][2 * u + 1], a.scale_log2, -ref)));
+            // the sum is over the rounded weights that multiply V
+            const float2 w = Tr::unpack2(p);
+            l[mt][u] += w.x + w.y;
+            const int key = warp * S::kKeys + i * 8;
+            *reinterpret_cast<uint32_t*>(smem + S::kP + swizzled(r, key / 8, kRows * 128) + c2 * 2) = p;
+          }
+        }
+      }
+      named_barrier_sync(1, kConsumers);
+      // O += P V for this warp's eighth of the values, 32 keys per step
+#pragma unroll
+      for (int kk = 0; kk < BN / 32; ++kk) {
+        uint32_t p[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          ldmatrix_x4(p[mt][0], p_at + swizzled(mt * 16 + lane % 16, kk * 4 + lane / 16, kRows * 128));
+          ldmatrix_x4(p[mt][1], p_at + swizzled(mt * 16 + lane % 16, kk * 4 + 2 + lane / 16, kRows * 128));
         }
 #pragma unroll
-        for (int d = 0; d < NB * 4; ++d) {
-          const int chunk = (d % 4) * 2 + vchunk;
+        for (int i = 0; i < NB; ++i) {
           uint32_t b[4];
-          ldmatrix_x4_trans(b, vtile + (d / 4) * S::kBlockBytes + vkey * 128 + ((chunk ^ (vkey % 8)) * 16));
-          mma_16816<T>(o[2 * d], p, b[0], b[1]);
-          mma_16816<T>(o[2 * d + 1], p, b[2], b[3]);
+          ldmatrix_x4_trans(b, vtile + swizzled(kk * 32 + lane, warp * NB + i, S::kBlockBytes));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma_16816<T>(o[mt][i], p[mt][0], b[0], b[1]);
+            mma_16816<T>(o[mt][i], p[mt][1], b[2], b[3]);
+          }
         }
       }
       __syncwarp();
@@ -358,88 +428,48 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
         phase ^= 1;
       }
     }
-    // ---- the warps' states as one: common maximum, scaled sums, then O pairwise in a fixed order
+    // the rows' sums over all warps (row_max's readers have passed the last barrier)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-      if (lane % 4 == 0) {
-        merge_m[warp * 16 + g + 8 * u] = m[u];
-        merge_l[warp * 16 + g + 8 * u] = l[u];
-      }
-    }
-    named_barrier_sync(1, NW * 32);
-    if (*abort_flag != 0) return;
-    float total[2], top[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      top[u] = -INFINITY;
-      for (int w = 0; w < NW; ++w) top[u] = fmaxf(top[u], merge_m[w * 16 + g + 8 * u]);
-      const float ref = top[u] == -INFINITY ? 0.f : top[u];
-      total[u] = 0.f;
-      for (int w = 0; w < NW; ++w) {
-        total[u] += merge_l[w * 16 + g + 8 * u] * fast_exp2(merge_m[w * 16 + g + 8 * u] - ref);
-      }
-      const float keep = fast_exp2(m[u] - ref);
-#pragma unroll
-      for (int i = 0; i < NB * 8; ++i) {
-        o[i][2 * u] *= keep;
-        o[i][2 * u + 1] *= keep;
-      }
-    }
-#pragma unroll
-    for (int half = NW / 2; half > 0; half /= 2) {
-      float* mine = merge_o + (warp % half) * 16 * S::kDim;
-      if (warp >= half && warp < 2 * half) {
-#pragma unroll
-        for (int i = 0; i < NB * 8; ++i) {
-          *reinterpret_cast<float2*>(mine + g * S::kDim + i * 8 + c2) = make_float2(o[i][0], o[i][1]);
-          *reinterpret_cast<float2*>(mine + (g + 8) * S::kDim + i * 8 + c2) = make_float2(o[i][2], o[i][3]);
-        }
-      }
-      named_barrier_sync(1, NW * 32);
-      if (warp < half) {
-#pragma unroll
-        for (int i = 0; i < NB * 8; ++i) {
-          const float2 x = *reinterpret_cast<float2*>(mine + g * S::kDim + i * 8 + c2);
-          const float2 y = *reinterpret_cast<float2*>(mine + (g + 8) * S::kDim + i * 8 + c2);
-          o[i][0] += x.x;
-          o[i][1] += x.y;
-          o[i][2] += y.x;
-          o[i][3] += y.y;
-        }
-      }
-      named_barrier_sync(1, NW * 32);
-    }
-    if (sg.slot < 0) {
-      if (warp == 0) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (row_o[u] < 0) continue;
-          const float inv = total[u] > 0.f ? 1.f / total[u] : 0.f;
-          T* out = static_cast<T*>(a.out) + row_o[u];
-#pragma unroll
-          for (int i = 0; i < NB * 8; ++i) {
-            if (i * 8 < a.dim) {
-              *reinterpret_cast<uint32_t*>(out + i * 8 + c2) = Tr::pack2(o[i][2 * u] * inv, o[i][2 * u + 1] * inv);
-            }
-          }
-        }
-      }
-      continue;
-    }
-    // A piece: normalised O and base-2 LSE to its slot
-    if (warp == 0) {
+    for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const long long at = static_cast<long long>(sg.slot) * kDecodeRows + g + 8 * u;
-        const float inv = total[u] > 0.f ? 1.f / total[u] : 0.f;
-        float* out = a.slots.o + at * a.dim;
+        l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 1);
+        l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 2);
+        if (lane % 4 == 0) row_max[(mt * 16 + g + 8 * u) * NW + warp] = l[mt][u];
+      }
+    }
+    named_barrier_sync(1, kConsumers);
 #pragma unroll
-        for (int i = 0; i < NB * 8; ++i) {
-          if (i * 8 < a.dim) *reinterpret_cast<float2*>(out + i * 8 + c2) = make_float2(o[i][2 * u] * inv, o[i][2 * u + 1] * inv);
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = mt * 16 + g + 8 * u;
+        const float4 t0 = *reinterpret_cast<const float4*>(&row_max[r * NW]);
+        const float4 t1 = *reinterpret_cast<const float4*>(&row_max[r * NW + 4]);
+        const float total = ((t0.x + t0.y) + (t0.z + t0.w)) + ((t1.x + t1.y) + (t1.z + t1.w));
+        const float inv = total > 0.f ? 1.f / total : 0.f;
+        if (sg.slot < 0) {
+          if (out_at[mt][u] < 0) continue;
+          T* out = static_cast<T*>(a.out) + out_at[mt][u];
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const int at = (warp * NB + i) * 8;
+            if (at >= a.dim) continue;
+            const float x = total > 0.f ? o[mt][i][2 * u] * inv : 0.f, y = total > 0.f ? o[mt][i][2 * u + 1] * inv : 0.f;
+            *reinterpret_cast<uint32_t*>(out + at + c2) = Tr::pack2(x, y);
+          }
+        } else {
+          // a piece: normalised O and base-2 LSE to its slot
+          const long long at_row = static_cast<long long>(sg.slot) * kRows + r;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const int at = (warp * NB + i) * 8;
+            if (at >= a.dim) continue;
+            const float x = total > 0.f ? o[mt][i][2 * u] * inv : 0.f, y = total > 0.f ? o[mt][i][2 * u + 1] * inv : 0.f;
+            *reinterpret_cast<float2*>(a.slots.o + at_row * a.dim + at + c2) = make_float2(x, y);
+          }
+          if (warp == 0 && lane % 4 == 0) a.slots.lse[at_row] = total > 0.f ? m[mt][u] + fast_log2(total) : kEmptyLse;
         }
-        if (lane % 4 == 0) a.slots.lse[at] = total[u] > 0.f ? top[u] + fast_log2(total[u]) : kEmptyLse;
       }
     }
     if (sg.starts && threadIdx.x == 0) {
@@ -449,10 +479,10 @@ __global__ void __launch_bounds__(DecodeShape<NB>::kThreads, 1)
   grid_dependency_wait();  // so that what follows this kernel follows the plan ahead of it too
 }
 
-template <typename T, int NB>
+template <typename T, int NB, int MT>
 static cudaError_t launch_decode_t(const fgw_chunk_params& p, ChunkArgs a, int device, cudaStream_t stream) {
-  using S = DecodeShape<NB>;
-  auto kernel = chunk_decode_kernel<T, NB>;
+  using S = DecodeShape<NB, MT>;
+  auto kernel = chunk_decode_kernel<T, NB, MT>;
   cudaError_t err = prepare_kernel(reinterpret_cast<const void*>(kernel), S::kBytes, device, nullptr);
   if (err != cudaSuccess) return err;
   a.box_rows = chunk_box_rows(p.page_size, S::kBN);
@@ -466,23 +496,36 @@ static cudaError_t launch_decode_t(const fgw_chunk_params& p, ChunkArgs a, int d
   return cudaGetLastError();
 }
 
-template <typename T>
+template <typename T, int NB>
 static cudaError_t launch_decode_nb(const fgw_chunk_params& p, const ChunkArgs& a, int device, cudaStream_t stream) {
+  switch (a.small_rows) {
+    case 16:
+      return launch_decode_t<T, NB, 1>(p, a, device, stream);
+    case 32:
+      return launch_decode_t<T, NB, 2>(p, a, device, stream);
+    default:
+      if constexpr (NB <= 2) return launch_decode_t<T, NB, 4>(p, a, device, stream);
+      return cudaErrorInvalidValue;
+  }
+}
+
+template <typename T>
+static cudaError_t launch_decode_type(const fgw_chunk_params& p, const ChunkArgs& a, int device, cudaStream_t stream) {
   switch ((p.head_dim + 63) / 64) {
     case 1:
-      return launch_decode_t<T, 1>(p, a, device, stream);
+      return launch_decode_nb<T, 1>(p, a, device, stream);
     case 2:
-      return launch_decode_t<T, 2>(p, a, device, stream);
+      return launch_decode_nb<T, 2>(p, a, device, stream);
     case 3:
-      return launch_decode_t<T, 3>(p, a, device, stream);
+      return launch_decode_nb<T, 3>(p, a, device, stream);
     default:
-      return launch_decode_t<T, 4>(p, a, device, stream);
+      return launch_decode_nb<T, 4>(p, a, device, stream);
   }
 }
 
 cudaError_t launch_chunk_decode(const fgw_chunk_params& p, ChunkArgs a, int device, cudaStream_t stream) {
-  return p.dtype == FGW_DTYPE_BFLOAT16 ? launch_decode_nb<__nv_bfloat16>(p, a, device, stream)
-                                       : launch_decode_nb<__half>(p, a, device, stream);
+  return p.dtype == FGW_DTYPE_BFLOAT16 ? launch_decode_type<__nv_bfloat16>(p, a, device, stream)
+                                       : launch_decode_type<__half>(p, a, device, stream);
 }
 
 }  // namespace fgw

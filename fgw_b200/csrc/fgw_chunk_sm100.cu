@@ -1,4 +1,4 @@
-// Chunk attention, tensor kernel (tcgen05): requests with more than 16 (token, query head) rows per key head.
+// Chunk attention, tensor kernel (tcgen05): the requests with more rows than a decode item.
 //
 // Rows of a 128-row tile are (token, query head of the group) pairs of one key head, token by token: 128 / G tokens of G
 // heads. One TMA box {64 values, G heads, 128 / G tokens} loads such a tile from the queries as they lie in memory, and

@@ -5,6 +5,9 @@ step brings single tokens and prompt chunks together, grouped heads, and lengths
 ``paged_chunk_attention`` takes those as they are: query head h reads key head h // (heads // kv_heads), request b's
 new tokens are rows ``cu_seqlens_q[b]`` to ``cu_seqlens_q[b + 1]``, and nothing is copied to the host.
 """
+import functools
+import struct
+
 import torch
 
 from fgw_b200 import _native
@@ -12,44 +15,51 @@ from fgw_b200.operators.mha.kernels.mha_paged_fwd_sm100 import _KEPT, _KEPT_WORK
 
 _DTYPES = {torch.float16: _native.DTYPE_FLOAT16, torch.bfloat16: _native.DTYPE_BFLOAT16}
 MAX_GROUP = 128  # query heads that may share a key head
+_PACK = struct.Struct(_native.struct_format(_native.ChunkParams)).pack  # one call instead of a store per field
 
 
 def check_ragged(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens_q, page_size):
-    """Checks shared by the operators over a ragged batch and a paged cache; returns (tokens, heads, dim, kv_heads)."""
-    if q.dim() != 3 or k_cache.dim() != 3 or v_cache.shape != k_cache.shape:
+    """Checks shared by the operators over a ragged batch and a paged cache; returns (tokens, heads, dim, kv_heads,
+    pool_rows, batch, width)."""
+    pool = k_cache.shape
+    if q.dim() != 3 or len(pool) != 3 or v_cache.shape != pool:
         raise ValueError("Expected q[T,H,D] and K/V[N,Hkv,D]")
     tokens, heads, dim = q.shape
-    kv_heads = k_cache.shape[1]
-    if k_cache.shape[2] != dim or kv_heads <= 0 or heads % kv_heads:
+    rows, kv_heads, pool_dim = pool
+    if pool_dim != dim or kv_heads <= 0 or heads <= 0 or heads % kv_heads:
         raise ValueError("K/V heads must divide the query heads and share their dimension")
-    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype not in _DTYPES or k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise ValueError("FP16 or BF16 required, the same for every tensor")
     if dim < 16 or dim > 256 or dim % 16:
         raise ValueError("D must be in [16, 256] and divisible by 16")
-    if page_size <= 0 or page_size % 16 or k_cache.shape[0] <= 0 or k_cache.shape[0] % page_size:
+    if page_size <= 0 or page_size % 16 or rows <= 0 or rows % page_size:
         raise ValueError("page_size must be a positive multiple of 16 and divide the pool's rows")
-    batch = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else 0
-    if (batch <= 0 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] <= 0
-            or cu_seqlens_q.shape != (batch + 1,)):
+    if block_table.dim() != 2:
+        raise ValueError("metadata shape mismatch")
+    batch, width = block_table.shape
+    if batch <= 0 or width <= 0 or cache_seqlens.shape != (batch,) or cu_seqlens_q.shape != (batch + 1,):
         raise ValueError("metadata shape mismatch")
     if not block_table.dtype == cache_seqlens.dtype == cu_seqlens_q.dtype == torch.int32:
         raise ValueError("page table, lengths and offsets must be int32")
-    if block_table.shape[1] * page_size > (1 << 31) - 1:
-        raise ValueError("requires logical positions to fit int32")
-    device = q.device
-    if not q.is_cuda or any(t.device != device for t in (k_cache, v_cache, block_table, cache_seqlens, cu_seqlens_q)):
+    if width * page_size > (1 << 31) - 1 or tokens > (1 << 31) - 1 or rows > (1 << 31) - 1:
+        raise ValueError("requires logical positions, tokens and pool rows to fit int32")
+    device = q.get_device()  # -1 on the CPU
+    if (device < 0 or k_cache.get_device() != device or v_cache.get_device() != device
+            or block_table.get_device() != device or cache_seqlens.get_device() != device
+            or cu_seqlens_q.get_device() != device):
         raise ValueError("every tensor must be on the same CUDA device")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and block_table.is_contiguous()
             and cache_seqlens.is_contiguous() and cu_seqlens_q.is_contiguous()):
         raise ValueError("kernel inputs must be contiguous")
-    return tokens, heads, dim, kv_heads
+    return tokens, heads, dim, kv_heads, rows, batch, width
 
 
 def token_stride(x, name):
     """Elements from one token's row to the next of ``x`` [tokens, heads, dim]; each row itself is contiguous."""
     tokens, heads, dim = x.shape
     stride, head_stride, one = x.stride()
-    if (one != 1 and dim > 1) or (head_stride != dim and heads > 1):
+    if one != 1 or (head_stride != dim and heads > 1):
         raise ValueError(f"{name}: a token's heads must be contiguous")
     if tokens <= 1:
         return heads * dim
@@ -58,12 +68,54 @@ def token_stride(x, name):
     return stride
 
 
-def aligned(x, name):
-    """The data pointer of ``x``; 16-byte aligned as the kernels' vector accesses and TMA need it."""
-    at = x.data_ptr()
-    if at % 16:
-        raise ValueError(f"{name} must be 16-byte aligned")
-    return at
+def aligned(*tensors):
+    """The data pointers; 16-byte aligned as the kernels' vector accesses and TMA need them."""
+    pointers = [t.data_ptr() for t in tensors]
+    if any([p & 15 for p in pointers]):
+        raise ValueError("tensors must be 16-byte aligned")
+    return pointers
+
+
+def output_like(q, out):
+    """``out``, or a new contiguous tensor of q's shape, and its token stride."""
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        return out, q.shape[1] * q.shape[2]
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must match q")
+    return out, token_stride(out, "out")
+
+
+def on_device(device, call, *args):
+    """``call(*args)`` with CUDA device index ``device`` current."""
+    if torch._C._cuda_getDevice() == device:
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(tokens, batch, heads, kv_heads, dim, page_size):
+    p = _native.ChunkParams()
+    p.tokens, p.batch, p.heads, p.kv_heads, p.head_dim = tokens, batch, heads, kv_heads, dim
+    p.pool_rows = p.page_size = page_size
+    p.table_width = 1
+    p.q_stride = p.out_stride = heads * dim
+    p.softmax_scale = 1.0
+    return _native.chunk_workspace_size(p)
+
+
+def _launch(params, nbytes, device):
+    stream = _current_stream(device)
+    # a graph keeps what it allocates while it is captured, and would outlive a kept workspace
+    if nbytes > _KEPT_WORKSPACE_BYTES or torch.cuda.is_current_stream_capturing():
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _native.chunk_attention(params, workspace.data_ptr(), nbytes, stream)
+        return
+    with _KEPT.lock:
+        workspace = _KEPT.get(("chunk", nbytes, device, stream), nbytes,
+                              lambda: torch.empty(nbytes, dtype=torch.uint8, device=device))
+        _native.chunk_attention(params, workspace.data_ptr(), nbytes, stream)
 
 
 def paged_chunk_attention(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens_q, page_size, is_causal=True,
@@ -76,40 +128,21 @@ def paged_chunk_attention(q, k_cache, v_cache, block_table, cache_seqlens, cu_se
     i-th of a request's n new tokens sees the first ``cache_seqlens - n + i + 1`` cached ones. Rows that see nothing and
     rows of no request are exact zeros. ``softmax_scale`` defaults to 1 / sqrt(D).
     """
-    tokens, heads, dim, kv_heads = check_ragged(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens_q,
-                                                page_size)
-    if heads // kv_heads > MAX_GROUP:
+    tokens, heads, dim, kv_heads, rows, batch, width = check_ragged(q, k_cache, v_cache, block_table, cache_seqlens,
+                                                                    cu_seqlens_q, page_size)
+    if heads > MAX_GROUP * kv_heads:
         raise ValueError(f"at most {MAX_GROUP} query heads per key head")
     scale = dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale <= 1e30:
         raise ValueError("softmax_scale must be positive and finite")
-    if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError("out must match q")
+    out, out_stride = output_like(q, out)
+    q_stride = token_stride(q, "q")
     if not tokens:
         return out
-    p = _native.ChunkParams()
-    p.q, p.k_cache, p.v_cache, p.out = (aligned(q, "q"), aligned(k_cache, "k_cache"), aligned(v_cache, "v_cache"),
-                                        aligned(out, "out"))
-    p.block_table, p.cache_seqlens = block_table.data_ptr(), cache_seqlens.data_ptr()
-    p.cu_seqlens_q = cu_seqlens_q.data_ptr()
-    p.tokens, p.pool_rows = tokens, k_cache.shape[0]
-    p.q_stride, p.out_stride = token_stride(q, "q"), token_stride(out, "out")
-    p.batch, p.heads, p.kv_heads, p.head_dim = cache_seqlens.shape[0], heads, kv_heads, dim
-    p.table_width, p.page_size = block_table.shape[1], page_size
-    p.dtype, p.causal, p.softmax_scale = _DTYPES[q.dtype], 1 if is_causal else 0, scale
-    device = q.device.index
-    nbytes = _native.chunk_workspace_size(p)
-    with torch.cuda.device(device):
-        stream = _current_stream(device)
-        # a graph keeps what it allocates while it is captured, and would outlive a kept workspace
-        if nbytes > _KEPT_WORKSPACE_BYTES or torch.cuda.is_current_stream_capturing():
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            _native.chunk_attention(p, workspace.data_ptr(), nbytes, stream)
-        else:
-            with _KEPT.lock:
-                workspace = _KEPT.get(("chunk", nbytes, device, stream), nbytes,
-                                      lambda: torch.empty(nbytes, dtype=torch.uint8, device=q.device))
-                _native.chunk_attention(p, workspace.data_ptr(), nbytes, stream)
+    q_at, k_at, v_at, out_at = aligned(q, k_cache, v_cache, out)
+    params = _PACK(q_at, k_at, v_at, block_table.data_ptr(), cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), out_at,
+                   tokens, rows, q_stride, out_stride, batch, heads, kv_heads, dim, width, page_size, _DTYPES[q.dtype],
+                   1 if is_causal else 0, scale, 0, 0, 0)
+    nbytes = _workspace_bytes(tokens, batch, heads, kv_heads, dim, page_size)
+    on_device(q.get_device(), _launch, params, nbytes, q.get_device())
     return out

@@ -5,14 +5,17 @@ keys and writes keys and values where ``paged_chunk_attention`` reads them, in o
 callers bring a filled cache.
 """
 import math
+import struct
 
 import torch
 
 from fgw_b200 import _native
-from fgw_b200.operators.mha.chunk_attention import _DTYPES, aligned, check_ragged, token_stride
+from fgw_b200.operators.mha.chunk_attention import (_DTYPES, aligned, check_ragged, on_device, output_like,
+                                                    token_stride)
 from fgw_b200.operators.mha.kernels.mha_paged_fwd_sm100 import _current_stream
 
 SCALINGS = (None, "linear", "ntk", "yarn")
+_PACK = struct.Struct(_native.struct_format(_native.RotaryParams)).pack
 
 
 def rotary_table(positions, rotary_dim, base=10000.0, scaling=None, factor=1.0, original_positions=None,
@@ -71,40 +74,29 @@ def rotary_append(q, k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seql
     ``interleaved``; values from rotary_dim on pass. ``out`` may be ``q``. Rows of no request, and positions outside
     the page table or ``cos_sin``, give zeros and append nothing.
     """
-    tokens, heads, dim, kv_heads = check_ragged(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens_q,
-                                                page_size)
+    tokens, heads, dim, kv_heads, rows, batch, width = check_ragged(q, k_cache, v_cache, block_table, cache_seqlens,
+                                                                    cu_seqlens_q, page_size)
     if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape:
         raise ValueError("Expected k and v [T,Hkv,D]")
     if k.dtype != q.dtype or v.dtype != q.dtype or cos_sin.dtype != torch.float32:
         raise ValueError("k and v take q's type, cos_sin float32")
-    if cos_sin.dim() != 2 or cos_sin.shape[0] <= 0:
+    if cos_sin.dim() != 2:
         raise ValueError("cos_sin must be [positions, rotary_dim]")
-    rotary_dim = cos_sin.shape[1]
-    if rotary_dim < 2 or rotary_dim > dim or rotary_dim % 2:
-        raise ValueError("rotary_dim must be even and at most D")
-    if any(t.device != q.device for t in (k, v, cos_sin)):
+    positions, rotary_dim = cos_sin.shape
+    if positions <= 0 or rotary_dim < 2 or rotary_dim > dim or rotary_dim % 2:
+        raise ValueError("cos_sin must have a row and rotary_dim be even and at most D")
+    device = q.get_device()
+    if k.get_device() != device or v.get_device() != device or cos_sin.get_device() != device:
         raise ValueError("every tensor must be on the same CUDA device")
     if not cos_sin.is_contiguous():
         raise ValueError("kernel inputs must be contiguous")
-    if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError("out must match q")
+    out, out_stride = output_like(q, out)
+    q_stride, k_stride, v_stride = token_stride(q, "q"), token_stride(k, "k"), token_stride(v, "v")
     if not tokens:
         return out
-    p = _native.RotaryParams()
-    p.q, p.k, p.v, p.q_out = aligned(q, "q"), aligned(k, "k"), aligned(v, "v"), aligned(out, "out")
-    p.k_cache, p.v_cache = aligned(k_cache, "k_cache"), aligned(v_cache, "v_cache")
-    p.block_table, p.cache_seqlens = block_table.data_ptr(), cache_seqlens.data_ptr()
-    p.cu_seqlens_q, p.cos_sin = cu_seqlens_q.data_ptr(), cos_sin.data_ptr()
-    p.tokens, p.pool_rows = tokens, k_cache.shape[0]
-    p.q_stride, p.k_stride = token_stride(q, "q"), token_stride(k, "k")
-    p.v_stride, p.q_out_stride = token_stride(v, "v"), token_stride(out, "out")
-    p.batch, p.heads, p.kv_heads, p.head_dim = cache_seqlens.shape[0], heads, kv_heads, dim
-    p.rotary_dim, p.positions = rotary_dim, min(cos_sin.shape[0], (1 << 31) - 1)
-    p.table_width, p.page_size = block_table.shape[1], page_size
-    p.dtype, p.interleaved = _DTYPES[q.dtype], 1 if interleaved else 0
-    device = q.device.index
-    with torch.cuda.device(device):
-        _native.rotary_append(p, _current_stream(device))
+    params = _PACK(*aligned(q, k, v, out, k_cache, v_cache), block_table.data_ptr(), cache_seqlens.data_ptr(),
+                   cu_seqlens_q.data_ptr(), cos_sin.data_ptr(), tokens, rows, q_stride, k_stride, v_stride, out_stride,
+                   batch, heads, kv_heads, dim, rotary_dim, min(positions, (1 << 31) - 1), width, page_size,
+                   _DTYPES[q.dtype], 1 if interleaved else 0, 0, 0)
+    on_device(device, _native.rotary_append, params, _current_stream(device))
     return out
