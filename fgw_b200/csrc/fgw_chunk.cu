@@ -22,7 +22,7 @@ constexpr int kPlanSorted = 2048;     // rows of a list sorted in shared memory;
 constexpr int kItemCost = 2;          // KV tiles that an item's start and end cost, in the choice of whole rounds
 constexpr int kTensorMinUnits = 2;    // units a program's range has at least when every item is cut
 constexpr int kMergeThreads = 256;
-constexpr int kMergeRows = 32;        // rows merged by one CTA
+constexpr int kMergeRows[2] = {8, 16};  // rows merged by one CTA, by list
 
 // Sum over the CTA of each thread's value before it in thread order, and the total.
 template <typename V>
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kPlanListThreads)
     const int len = held_tokens(a.lens, b, a.width, a.page);
     for (int r = begin + lane; r < end; r += 32) {
       const int t0 = (r - begin) * a.tokens_per_item;
-      raw[r] = make_int4(b, t0, item_units(a, count, len, t0), 0);
+      raw[r] = make_int4(b, t0, item_units<128>(a, count, len, t0), 0);
     }
   }
   __syncthreads();
@@ -195,13 +195,14 @@ __global__ void __launch_bounds__(kPlanListThreads)
   }
 }
 
-// Merges the pieces of the cut items of both kernels, kMergeRows rows per CTA: the weights 2^(lse - peak) of all pieces
-// first, in shared memory, then the weighted sum of their O in piece order with independent loads. Also writes zeros
-// into the rows of no request and reduces the CTAs' errors to the header's word.
+// Merges the pieces of the cut items of both kernels, a few rows per CTA, every thread four values of one row: a
+// running peak of the pieces' LSEs, their weights 2^(lse - peak) and the weighted sum, in piece order, eight pieces'
+// loads at a time. Bound by the latency of two dependent trips to L2 (the cut, then its pieces). Also writes zeros into the
+// rows of no request and reduces the CTAs' errors to the header's word.
 struct MergeList {
   ChunkSlots slots;
   const long long* prog_u;  // [programs + 1]: programs without units hold no piece (nullptr: all hold one)
-  int slot_rows, parts;     // parts CTAs per program
+  int slot_rows, rows, parts;  // `parts` CTAs per program, `rows` rows each
   bool by_column;           // O laid out [dim / 4][rows][4], else [rows][dim]
 };
 struct MergeArgs {
@@ -210,39 +211,100 @@ struct MergeArgs {
   MergeList list[2];  // decode, tensor; parts 0: kernel not launched
 };
 
+__device__ void merge_errors(const MergeArgs& m) {
+  int code = 0, site = 0;
+  for (int k = 0; k < 2; ++k) {
+    for (int p = threadIdx.x; m.list[k].parts > 0 && p < m.a.programs; p += 32) {
+      const int2 e = m.list[k].slots.errors[p];
+      if (e.x != 0 && code == 0) {
+        code = e.x;
+        site = e.y;
+      }
+    }
+  }
+  const uint32_t any = __ballot_sync(0xffffffffu, code != 0);
+  const int from = any != 0 ? __ffs(any) - 1 : 0;
+  code = __shfl_sync(0xffffffffu, code, from);
+  site = __shfl_sync(0xffffffffu, site, from);
+  if (threadIdx.x == 0) {
+    m.ws->error = code;
+    m.ws->error_site = site;
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid_constant__ MergeArgs m) {
   using Tr = ElemTraits<T>;
-  __shared__ float weight[kStreamMaxPrograms][kMergeRows];
-  __shared__ float inverse[kMergeRows];
-  __shared__ int slot[kStreamMaxPrograms];
-  __shared__ int pieces_s;
   const ChunkArgs& a = m.a;
-  grid_dependency_wait();
   const int tid = threadIdx.x;
-  if (blockIdx.x == 0 && tid < 32) {
-    int code = 0, site = 0;
-    for (int k = 0; k < 2; ++k) {
-      for (int p = tid; m.list[k].parts > 0 && p < a.programs; p += 32) {
-        const int2 e = m.list[k].slots.errors[p];
-        if (e.x != 0 && code == 0) {
-          code = e.x;
-          site = e.y;
+  const int decode_ctas = m.list[0].parts * a.programs;
+  const int kind = static_cast<int>(blockIdx.x) < decode_ctas ? 0 : 1;
+  const MergeList& l = m.list[kind];
+  const int at = blockIdx.x - (kind ? decode_ctas : 0);
+  const int q = at / l.parts, row0 = at % l.parts * l.rows;
+  const int groups = a.dim / 4;
+  const int tile_tokens = kTensorTileRows / a.group;
+  const long long step = static_cast<long long>(l.slot_rows) * groups;  // float4s of a slot
+  grid_dependency_wait();
+  const ChunkCut cut = l.slots.cuts[q];
+  const long long first = min(max(static_cast<long long>(a.cu[0]), 0ll), a.tokens);
+  const long long end = min(max(static_cast<long long>(a.cu[a.batch]), first), a.tokens);
+  if (cut.last >= q) {
+    for (int i = tid; i < l.rows * groups; i += kMergeThreads) {
+      // neighbouring threads read neighbouring 16 bytes of the slot
+      const int r = l.by_column ? i % l.rows : i / groups, g = l.by_column ? i / l.rows : i % groups;
+      const int row = row0 + r;
+      // a slot's rows are (tile, row of the tile); a tile holds whole tokens
+      const int tile = row / kTensorTileRows, in_tile = row % kTensorTileRows;
+      const int in_token = a.by_group.quotient(in_tile), token = tile * tile_tokens + in_token;
+      if (row >= l.slot_rows || in_token >= tile_tokens || token >= cut.count) continue;
+      const float4* src = reinterpret_cast<const float4*>(l.slots.o) +
+                          (l.by_column ? static_cast<long long>(g) * l.slot_rows + row : static_cast<long long>(row) * groups + g);
+      const float* lses = l.slots.lse + row;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float peak = kEmptyLse, sum = 0.f;
+      for (int p0 = q; p0 <= cut.last; p0 += 8) {
+        float4 v[8];
+        float w[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int p = p0 + u;
+          w[u] = kEmptyLse;
+          v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (p <= cut.last && (l.prog_u == nullptr || l.prog_u[p] < l.prog_u[p + 1])) {
+            const int slot = 2 * p + (p == q ? 1 : 0);
+            w[u] = lses[static_cast<long long>(slot) * l.slot_rows];
+            v[u] = src[slot * step];
+          }
+        }
+        float next = peak;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) next = fmaxf(next, w[u]);
+        const float keep = fast_exp2(peak - next);
+        sum *= keep;
+        acc.x *= keep;
+        acc.y *= keep;
+        acc.z *= keep;
+        acc.w *= keep;
+        peak = next;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float wk = w[u] > kValidLse ? fast_exp2(w[u] - peak) : 0.f;
+          sum += wk;
+          acc.x = fmaf(wk, v[u].x, acc.x);
+          acc.y = fmaf(wk, v[u].y, acc.y);
+          acc.z = fmaf(wk, v[u].z, acc.z);
+          acc.w = fmaf(wk, v[u].w, acc.w);
         }
       }
-    }
-    const uint32_t any = __ballot_sync(0xffffffffu, code != 0);
-    const int from = any != 0 ? __ffs(any) - 1 : 0;
-    code = __shfl_sync(0xffffffffu, code, from);
-    site = __shfl_sync(0xffffffffu, site, from);
-    if (tid == 0) {
-      m.ws->error = code;
-      m.ws->error_site = site;
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      T* out = static_cast<T*>(a.out) + (cut.token0 + token) * a.out_stride +
+               static_cast<long long>(cut.hk * a.group + in_tile - in_token * a.group) * a.dim + g * 4;
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(Tr::pack2(acc.x * inv, acc.y * inv), Tr::pack2(acc.z * inv, acc.w * inv));
     }
   }
   // rows of no request
-  const long long first = min(max(static_cast<long long>(a.cu[0]), 0ll), a.tokens);
-  const long long end = min(max(static_cast<long long>(a.cu[a.batch]), first), a.tokens);
   const int chunks = a.heads * a.dim / 8;
   const long long none = (first + a.tokens - end) * chunks;
   for (long long i = static_cast<long long>(blockIdx.x) * kMergeThreads + tid; i < none;
@@ -251,76 +313,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
     const long long t = k < first ? k : end + k - first;
     reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + t * a.out_stride)[i % chunks] = make_uint4(0, 0, 0, 0);
   }
-  const int decode_ctas = m.list[0].parts * a.programs;
-  const int kind = static_cast<int>(blockIdx.x) < decode_ctas ? 0 : 1;
-  const MergeList& l = m.list[kind];
-  const int at = blockIdx.x - (kind ? decode_ctas : 0);
-  const int q = at / l.parts, row0 = at % l.parts * kMergeRows;
-  const ChunkCut cut = l.slots.cuts[q];
-  // rows of the slot are (tile, row of the tile) for the tensor kernel: tile 1 starts at row 128 whatever the group
-  const int tile_rows = kTensorTileRows / a.group * a.group;
-  if (cut.last < q) return;
-  if (tid == 0) {
-    int n = 0;
-    for (int p = q; p <= cut.last; ++p) {
-      if (l.prog_u == nullptr || l.prog_u[p] < l.prog_u[p + 1]) slot[n++] = 2 * p + (p == q ? 1 : 0);
-    }
-    pieces_s = n;
-  }
-  __syncthreads();
-  const int pieces = pieces_s;
-  for (int i = tid; i < pieces * kMergeRows; i += kMergeThreads) {
-    const int k = i / kMergeRows, r = i % kMergeRows;
-    const bool in = row0 + r < l.slot_rows;
-    weight[k][r] = in ? l.slots.lse[static_cast<long long>(slot[k]) * l.slot_rows + row0 + r] : kEmptyLse;
-  }
-  __syncthreads();
-  if (tid < kMergeRows) {
-    float peak = kEmptyLse, sum = 0.f;
-    for (int k = 0; k < pieces; ++k) peak = fmaxf(peak, weight[k][tid]);
-    for (int k = 0; k < pieces; ++k) {
-      const float lse = weight[k][tid];
-      const float w = lse > kValidLse ? fast_exp2(lse - peak) : 0.f;
-      weight[k][tid] = w;
-      sum += w;
-    }
-    inverse[tid] = sum > 0.f ? 1.f / sum : 0.f;
-  }
-  __syncthreads();
-  const int groups = a.dim / 4;
-  for (int i = tid; i < kMergeRows * groups; i += kMergeThreads) {
-    // neighbouring threads read neighbouring 16 bytes of the slot
-    const int r = l.by_column ? i % kMergeRows : i / groups, g = l.by_column ? i / kMergeRows : i % groups;
-    const int row = row0 + r;
-    const int tile = row / kTensorTileRows, in_tile = row % kTensorTileRows;
-    const int token = tile * (kTensorTileRows / a.group) + in_tile / a.group;
-    if (row >= l.slot_rows || in_tile >= tile_rows || token >= cut.count) continue;
-    const long long step = static_cast<long long>(l.slot_rows) * groups;  // float4s of a slot
-    const float4* src = reinterpret_cast<const float4*>(l.slots.o) +
-                        (l.by_column ? static_cast<long long>(g) * l.slot_rows + row : static_cast<long long>(row) * groups + g);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < pieces; k0 += 8) {
-      float4 v[8];
-      float w[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        w[u] = k0 + u < pieces ? weight[k0 + u][r] : 0.f;
-        v[u] = w[u] != 0.f ? src[slot[k0 + u] * step] : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        acc.x = fmaf(w[u], v[u].x, acc.x);
-        acc.y = fmaf(w[u], v[u].y, acc.y);
-        acc.z = fmaf(w[u], v[u].z, acc.z);
-        acc.w = fmaf(w[u], v[u].w, acc.w);
-      }
-    }
-    const float inv = inverse[r];
-    T* out = static_cast<T*>(a.out) + (cut.token0 + token) * a.out_stride +
-             static_cast<long long>(cut.hk * a.group + in_tile % a.group) * a.dim + g * 4;
-    *reinterpret_cast<uint2*>(out) =
-        make_uint2(Tr::pack2(acc.x * inv, acc.y * inv), Tr::pack2(acc.z * inv, acc.w * inv));
-  }
+  if (blockIdx.x == 0 && tid < 32) merge_errors(m);
 }
 
 int chunk_validate(const fgw_chunk_params& p) {
@@ -389,7 +382,7 @@ static bool tensor_on(const fgw_chunk_params& p) {
 // The workspace from `at` on (sizes alone when it is null), by class: slots of both kernels, the tensor kernel's list.
 struct ChunkLayout {
   ChunkSlots slots[2];
-  int tokens_per_item[2], keys_per_unit[2], slot_rows[2];
+  int tokens_per_item[2], slot_rows[2];
   ChunkList list;
   size_t bytes;
 };
@@ -407,10 +400,8 @@ static ChunkLayout chunk_layout(const fgw_chunk_params& p, uint8_t* const begin)
   const size_t programs = kStreamMaxPrograms;
   const bool on[2] = {decode_on(p), tensor_on(p)};
   l.tokens_per_item[0] = decode_rows(p) / group;
-  l.keys_per_unit[0] = chunk_decode_keys(nb, decode_rows(p) / 16);
   l.slot_rows[0] = decode_rows(p);
   l.tokens_per_item[1] = kTensorTileRows / group * chunk_tensor_tiles(nb);
-  l.keys_per_unit[1] = 128;
   l.slot_rows[1] = kTensorTileRows * chunk_tensor_tiles(nb);
   for (int k = 0; k < 2; ++k) {
     if (!on[k]) continue;
@@ -459,6 +450,8 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_coun
   a[0].page = p.page_size;
   a[0].causal = p.causal;
   a[0].programs = std::min(sm_count, kStreamMaxPrograms);
+  a[0].by_page = FastDiv(p.page_size);
+  a[0].by_group = FastDiv(a[0].group);
   a[0].small_rows = decode_rows(p);
   a[0].split = on[0] && on[1] ? 1 : 0;
   a[0].scale_log2 = p.softmax_scale * kLog2e;
@@ -468,12 +461,13 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_coun
   merge.ws = static_cast<WorkspaceHeader*>(workspace);
   for (int k = 0; k < 2; ++k) {
     a[k].tokens_per_item = layout.tokens_per_item[k];
-    a[k].keys_per_unit = layout.keys_per_unit[k];
+    a[k].by_item_tokens = FastDiv(layout.tokens_per_item[k]);
     a[k].slots = layout.slots[k];
     if (!on[k]) continue;
     merge.list[k].slots = layout.slots[k];
     merge.list[k].slot_rows = layout.slot_rows[k];
-    merge.list[k].parts = (layout.slot_rows[k] + kMergeRows - 1) / kMergeRows;
+    merge.list[k].rows = kMergeRows[k];
+    merge.list[k].parts = (layout.slot_rows[k] + kMergeRows[k] - 1) / kMergeRows[k];
     merge.list[k].by_column = k == 1;
     merge.list[k].prog_u = k == 1 ? layout.list.prog_u : nullptr;
   }

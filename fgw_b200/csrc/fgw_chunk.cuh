@@ -48,6 +48,27 @@ struct ChunkList {
   int max_rows;
 };
 
+// Division of 0 <= n < 2^31 by a fixed positive number with a multiplication and shifts (Granlund and Montgomery, "Division
+// by invariant integers using multiplication", 1994): m = floor(2^32 (2^l - d) / d) + 1 with 2^l >= d, q = (t + (n - t) / 2)
+// / 2^(l - 1) with t = floor(m n / 2^32). A division by a variable takes some 150 cycles, and the kernels' starts are
+// chains of them.
+struct FastDiv {
+  uint32_t mul, shift, one;  // one: the divisor is 1
+  int by;
+  FastDiv() = default;
+  explicit FastDiv(int d) : by(d) {
+    uint32_t l = 0;
+    while (l < 31 && (1u << l) < static_cast<uint32_t>(d)) ++l;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+    shift = l > 0 ? l - 1 : 0;
+    one = l == 0;
+  }
+  __device__ __forceinline__ int quotient(int n) const {
+    const uint32_t u = static_cast<uint32_t>(n), t = __umulhi(mul, u);
+    return one ? n : static_cast<int>((t + ((u - t) >> 1)) >> shift);
+  }
+};
+
 struct ChunkArgs {
   void* out;
   const int32_t* table;
@@ -56,7 +77,8 @@ struct ChunkArgs {
   const void* q;
   long long tokens, q_stride, out_stride;
   int batch, heads, kv_heads, group, dim, width, page, causal, box_rows, programs;
-  int tokens_per_item, keys_per_unit;
+  int tokens_per_item;
+  FastDiv by_page, by_group, by_item_tokens;
   int small_rows;  // rows of a decode item; requests of at most so many go to the decode kernel
   int split;       // requests go by their rows; otherwise everything is the launched kernel's
   float scale_log2;
@@ -86,14 +108,15 @@ __device__ __forceinline__ int held_tokens(const int32_t* lens, int b, int width
 // Rows of the request's list, 0 when it belongs to the other kernel.
 __device__ __forceinline__ int item_rows(const ChunkArgs& a, int count, bool decode) {
   if (a.split && (count * a.group <= a.small_rows) != decode) return 0;
-  return (count + a.tokens_per_item - 1) / a.tokens_per_item;
+  return a.by_item_tokens.quotient(count + a.tokens_per_item - 1);
 }
 
 // KV tiles of the item that starts at the request's token t0; one without keys still costs one (zeros to write).
+template <int kKeys>
 __device__ __forceinline__ int item_units(const ChunkArgs& a, int count, int len, int t0) {
   const int last = min(t0 + a.tokens_per_item, count) - 1;
   const int seen = max(a.causal ? len - count + last + 1 : len, 0);
-  return max((seen + a.keys_per_unit - 1) / a.keys_per_unit, 1);
+  return max((seen + kKeys - 1) / kKeys, 1);
 }
 
 // One run of KV tiles of one item processed by this CTA: a whole item, or a piece of one cut between programs.
@@ -110,16 +133,16 @@ struct ChunkSegment {
 };
 
 // Fills in the segment of `count` units from `first` on of an item.
+template <int kKeys>
 __device__ __forceinline__ void make_segment(const ChunkArgs& a, ChunkSegment& s, int b, int hk, const NewTokens& nt,
-                                             int t0, int units, int first, int count) {
-  const int len = held_tokens(a.lens, b, a.width, a.page);
+                                             int len, int t0, int units, int first, int count) {
   s.b = b;
   s.hk = hk;
   s.token0 = nt.first + t0;
   s.count = min(a.tokens_per_item, nt.count - t0);
   s.seen0 = a.causal ? len - nt.count + t0 + 1 : len;
   s.limit = max(a.causal ? s.seen0 + s.count - 1 : len, 0);
-  const int tiles = (s.limit + a.keys_per_unit - 1) / a.keys_per_unit;
+  const int tiles = (s.limit + kKeys - 1) / kKeys;
   s.n_begin = first;
   s.n = max(0, min(first + count, tiles) - first);
   // a piece that starts inside its item is its program's first, one that starts the item its program's last

@@ -13,10 +13,8 @@
 //
 // The work is split without a plan kernel: every CTA sums the units of all requests and finds the start of its own
 // range. That costs two or three trips to L2 before the first load; a plan launch ahead of it measured 6 us more.
-//
-// Rows of V from the last visible key on hold whatever the ring or the page holds: the warp zeroes them, since a zero
-// weight times NaN would still be NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "fgw_chunk.cuh"
 
@@ -83,28 +81,50 @@ __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t 
 struct DecodeCursor {
   int b, row, hk, off;   // next item and the units of it before the range
   long long u, u_end;    // units left
-  long long total;       // units of all items, over so many programs
-  int programs;
+  long long quotient;    // every program's units, the first `remainder` have one more
+  int remainder;
 };
 
+// x / y for x >= 0 and y > 0; nearly always the cheap 32-bit one.
+__device__ __forceinline__ long long divide(long long x, int y) {
+  if (x <= 0x7fffffffll) return static_cast<long long>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
+  return x / y;
+}
+// First unit of program p (program_start with the quotient already taken).
+__device__ __forceinline__ long long range_start(long long quotient, int remainder, int p) {
+  return quotient * p + min(p, remainder);
+}
+
+// The program that holds unit u.
+__device__ __forceinline__ int range_of(const DecodeCursor& k, long long u) {
+  const long long longer = k.remainder * (k.quotient + 1);
+  if (u < longer) return static_cast<int>(divide(u, static_cast<int>(k.quotient) + 1));
+  return k.remainder + static_cast<int>(divide(u - longer, static_cast<int>(k.quotient)));
+}
+
 // Units of request b's items for one key head.
+template <int kKeys>
 __device__ __forceinline__ long long request_units(const ChunkArgs& a, int b) {
   const NewTokens nt = new_tokens(a.cu, a.tokens, b);
-  const int rows = item_rows(a, nt.count, true);
   const int len = held_tokens(a.lens, b, a.width, a.page);
+  const int rows = item_rows(a, nt.count, true);
   long long units = 0;
-  for (int r = 0; r < rows; ++r) units += item_units(a, nt.count, len, r * a.tokens_per_item);
+  for (int r = 0; r < rows; ++r) units += item_units<kKeys>(a, nt.count, len, r * a.tokens_per_item);
   return units;
 }
 
 // Thread t takes the t-th of kThreads equal runs of requests, so one sum over the CTA gives the total and one over the
 // threads before it the run that holds the range's start, which its thread then walks.
-template <int kThreads>
-__device__ DecodeCursor decode_cursor(const ChunkArgs& a, long long* shared, DecodeCursor* found) {
-  const int run = (a.batch + kThreads - 1) / kThreads;
+template <int kThreads, int kKeys>
+__device__ __forceinline__ DecodeCursor decode_cursor(const ChunkArgs& a, long long* shared, DecodeCursor* found) {
+  const int run = a.batch <= kThreads ? 1 : (a.batch + kThreads - 1) / kThreads;
   const int begin = min(static_cast<int>(threadIdx.x) * run, a.batch), end = min(begin + run, a.batch);
-  long long mine = 0;
-  for (int b = begin; b < end; ++b) mine += request_units(a, b);
+  long long first_units = 0, mine = 0;
+  for (int b = begin; b < end; ++b) {
+    const long long units = request_units<kKeys>(a, b);
+    if (b == begin) first_units = units;
+    mine += units;
+  }
   mine *= a.kv_heads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long before = mine;
@@ -125,32 +145,33 @@ __device__ DecodeCursor decode_cursor(const ChunkArgs& a, long long* shared, Dec
   before += base - mine;  // units of the runs before this one
   const int programs = static_cast<int>(max(1ll, min(static_cast<long long>(a.programs), total / kDecodeMinUnits)));
   const int p = blockIdx.x;
-  if (p < programs) {
-    const long long u = program_start(total, programs, p), u_end = program_start(total, programs, p + 1);
-    if (u < u_end && before <= u && u < before + mine) {
-      long long left = u - before;
-      int b = begin;
-      long long units = request_units(a, b);
-      while (left >= units * a.kv_heads) {
-        left -= units * a.kv_heads;
-        units = request_units(a, ++b);
-      }
-      const NewTokens nt = new_tokens(a.cu, a.tokens, b);
-      const int len = held_tokens(a.lens, b, a.width, a.page);
-      int row = 0;
-      long long w = item_units(a, nt.count, len, 0);
-      while (left >= w * a.kv_heads) {
-        left -= w * a.kv_heads;
-        ++row;
-        w = item_units(a, nt.count, len, row * a.tokens_per_item);
-      }
-      *found = {b, row, static_cast<int>(left / w), static_cast<int>(left % w), u, u_end, total, programs};
+  const long long quotient = divide(total, programs);
+  const int remainder = static_cast<int>(total - quotient * programs);
+  const long long u = range_start(quotient, remainder, p), u_end = range_start(quotient, remainder, p + 1);
+  if (p < programs && u < u_end && before <= u && u < before + mine) {
+    long long left = u - before, units = first_units;
+    int b = begin;
+    while (left >= units * a.kv_heads) {
+      left -= units * a.kv_heads;
+      units = request_units<kKeys>(a, ++b);
     }
+    const NewTokens nt = new_tokens(a.cu, a.tokens, b);
+    const int len = held_tokens(a.lens, b, a.width, a.page);
+    int row = 0;
+    int w = item_units<kKeys>(a, nt.count, len, 0);
+    while (left >= static_cast<long long>(w) * a.kv_heads) {
+      left -= static_cast<long long>(w) * a.kv_heads;
+      ++row;
+      w = item_units<kKeys>(a, nt.count, len, row * a.tokens_per_item);
+    }
+    const int hk = static_cast<int>(divide(left, w));
+    *found = {b, row, hk, static_cast<int>(left - static_cast<long long>(hk) * w), u, u_end, quotient, remainder};
   }
   __syncthreads();
   return *found;
 }
 
+template <int kKeys>
 __device__ __forceinline__ bool next_segment(const ChunkArgs& a, DecodeCursor& k, ChunkSegment& s) {
   if (k.u >= k.u_end) return false;
   NewTokens nt = new_tokens(a.cu, a.tokens, k.b);
@@ -160,9 +181,10 @@ __device__ __forceinline__ bool next_segment(const ChunkArgs& a, DecodeCursor& k
     nt = new_tokens(a.cu, a.tokens, k.b);
   }
   const int t0 = k.row * a.tokens_per_item;
-  const int units = item_units(a, nt.count, held_tokens(a.lens, k.b, a.width, a.page), t0);
+  const int len = held_tokens(a.lens, k.b, a.width, a.page);
+  const int units = item_units<kKeys>(a, nt.count, len, t0);
   const int count = static_cast<int>(min(static_cast<long long>(units - k.off), k.u_end - k.u));
-  make_segment(a, s, k.b, k.hk, nt, t0, units, k.off, count);
+  make_segment<kKeys>(a, s, k.b, k.hk, nt, len, t0, units, k.off, count);
   s.end_u = k.u - k.off + units;
   k.u += count;
   k.off += count;
@@ -174,6 +196,11 @@ __device__ __forceinline__ bool next_segment(const ChunkArgs& a, DecodeCursor& k
     }
   }
   return true;
+}
+
+// Mask of a register of two 16-bit V values, of keys `key` and `key + 1`, that keeps those below the limit.
+__device__ __forceinline__ uint32_t kept_keys(int key, int limit) {
+  return key + 1 < limit ? 0xffffffffu : (key < limit ? 0x0000ffffu : 0u);
 }
 
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile of 128-byte rows, blocks of 64 values `block` bytes apart,
@@ -198,18 +225,22 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
   __shared__ long long scan[S::kThreads / 32];
   __shared__ DecodeCursor found;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == NW * 32) {
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], NW);
     }
     *abort_flag = 0;
     fence_barrier_init();
+  }
+  if (threadIdx.x == 0) {
     a.slots.errors[blockIdx.x] = make_int2(0, 0);
     a.slots.cuts[blockIdx.x] = {0, 0, 0, -1};
   }
   grid_dependents_launch();
-  DecodeCursor cur = decode_cursor<S::kThreads>(a, scan, &found);  // with barriers of the whole CTA
+  DecodeCursor cur = decode_cursor<S::kThreads, BN>(a, scan, &found);  // with barriers of the whole CTA
   ChunkSegment sg;
 
   if (warp == NW) {
@@ -222,12 +253,13 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
     const uint64_t policy = l2_policy_evict_first();
     bool ok = true;
     uint32_t st = 0, phase = 0;
-    while (ok && next_segment(a, cur, sg)) {
+    while (ok && next_segment<BN>(a, cur, sg)) {
       const int32_t* table = a.table + static_cast<long long>(sg.b) * a.width;
       for (int j = 0; j < sg.n && ok; ++j) {
         const int tok = (sg.n_begin + j) * BN + box * a.box_rows;
         const bool load = which < 2 && tok < sg.limit;
-        const int row = load ? table[tok / a.page] * a.page + tok % a.page : 0;
+        const int page = a.by_page.quotient(tok);
+        const int row = load ? table[page] * a.page + tok - page * a.page : 0;
         const int loads = __popc(__ballot_sync(0xffffffffu, load));
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], phase ^ 1, a.budget_ns));
         if (!ok) {
@@ -255,17 +287,17 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
   const uint32_t base = smem_u32(smem);
   const uint32_t q_at = base + S::kQ, p_at = base + S::kP;
   uint32_t st = 0, phase = 0;
-  while (next_segment(a, cur, sg)) {
+  while (next_segment<BN>(a, cur, sg)) {
     int seen[MT][2];
     long long out_at[MT][2];  // element offset of the row's output, -1: no row
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int r = mt * 16 + g + 8 * u, i = r / a.group;
+        const int r = mt * 16 + g + 8 * u, i = a.by_group.quotient(r);
         const bool valid = i < sg.count;
         seen[mt][u] = valid ? seen_keys(a, sg, i) : 0;
-        out_at[mt][u] = valid ? (sg.token0 + i) * a.out_stride + static_cast<long long>(sg.hk * a.group + r % a.group) * a.dim
+        out_at[mt][u] = valid ? (sg.token0 + i) * a.out_stride + static_cast<long long>(sg.hk * a.group + r - i * a.group) * a.dim
                               : -1;
       }
     }
@@ -283,8 +315,9 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
       const int r = i / (S::kDim / 8), chunk = i % (S::kDim / 8);
       uint4 x = make_uint4(0, 0, 0, 0);
       if (r < sg.count * a.group && chunk * 8 < a.dim) {
-        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (sg.token0 + r / a.group) * a.q_stride +
-                                                 static_cast<long long>(sg.hk * a.group + r % a.group) * a.dim) + chunk);
+        const int t = a.by_group.quotient(r);
+        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (sg.token0 + t) * a.q_stride +
+                                                 static_cast<long long>(sg.hk * a.group + r - t * a.group) * a.dim) + chunk);
       }
       *reinterpret_cast<uint4*>(smem + S::kQ + swizzled(r, chunk, kRows * 128)) = x;
     }
@@ -356,18 +389,6 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
           if (lane % 4 == 0) row_max[(mt * 16 + g + 8 * u) * NW + warp] = top;
         }
       }
-      if (key0 + S::kKeys > sg.limit) {
-        // V rows past the last visible key hold whatever the ring or the page holds, and a zero weight times NaN is NaN
-        if (lane < S::kKeys && key0 + lane >= sg.limit) {
-          uint8_t* row = smem + (2 * st + 1) * S::kTileBytes + (warp * S::kKeys + lane) * 128;
-#pragma unroll
-          for (int blk = 0; blk < NB; ++blk) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(row + blk * S::kBlockBytes + c * 16) = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_proxy_async_smem();  // the ring's next TMA write to these rows comes after
-      }
       named_barrier_sync(1, kConsumers);
       if (*abort_flag != 0) return;  // all warps read it here, between the same two barriers
 #pragma unroll
@@ -401,25 +422,38 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
         }
       }
       named_barrier_sync(1, kConsumers);
-      // O += P V for this warp's eighth of the values, 32 keys per step
+      // O += P V for this warp's eighth of the values, 32 keys per step. V rows past the last visible key hold whatever
+      // the ring or the page holds, and a zero weight times NaN is NaN: an item's last tile zeroes them as operands.
+      const int tile0 = (sg.n_begin + j) * BN;
+      auto weigh = [&](auto tail) {
 #pragma unroll
-      for (int kk = 0; kk < BN / 32; ++kk) {
-        uint32_t p[MT][2][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          ldmatrix_x4(p[mt][0], p_at + swizzled(mt * 16 + lane % 16, kk * 4 + lane / 16, kRows * 128));
-          ldmatrix_x4(p[mt][1], p_at + swizzled(mt * 16 + lane % 16, kk * 4 + 2 + lane / 16, kRows * 128));
-        }
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          uint32_t b[4];
-          ldmatrix_x4_trans(b, vtile + swizzled(kk * 32 + lane, warp * NB + i, S::kBlockBytes));
+        for (int kk = 0; kk < BN / 32; ++kk) {
+          uint32_t p[MT][2][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            mma_16816<T>(o[mt][i], p[mt][0], b[0], b[1]);
-            mma_16816<T>(o[mt][i], p[mt][1], b[2], b[3]);
+            ldmatrix_x4(p[mt][0], p_at + swizzled(mt * 16 + lane % 16, kk * 4 + lane / 16, kRows * 128));
+            ldmatrix_x4(p[mt][1], p_at + swizzled(mt * 16 + lane % 16, kk * 4 + 2 + lane / 16, kRows * 128));
+          }
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, vtile + swizzled(kk * 32 + lane, warp * NB + i, S::kBlockBytes));
+            if constexpr (decltype(tail)::value) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) b[k] &= kept_keys(tile0 + kk * 32 + k * 8 + c2, sg.limit);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma_16816<T>(o[mt][i], p[mt][0], b[0], b[1]);
+              mma_16816<T>(o[mt][i], p[mt][1], b[2], b[3]);
+            }
           }
         }
+      };
+      if (tile0 + BN > sg.limit) {
+        weigh(std::true_type{});
+      } else {
+        weigh(std::false_type{});
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
@@ -473,7 +507,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
       }
     }
     if (sg.starts && threadIdx.x == 0) {
-      a.slots.cuts[blockIdx.x] = {sg.token0, sg.count, sg.hk, program_of(cur.total, cur.programs, sg.end_u - 1)};
+      a.slots.cuts[blockIdx.x] = {sg.token0, sg.count, sg.hk, range_of(cur, sg.end_u - 1)};
     }
   }
   grid_dependency_wait();  // so that what follows this kernel follows the plan ahead of it too
