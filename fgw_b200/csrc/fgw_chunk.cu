@@ -19,7 +19,8 @@ namespace fgw {
 
 constexpr int kPlanListThreads = 1024;
 constexpr int kPlanSorted = 2048;     // rows of a list sorted in shared memory; longer lists keep the request order
-constexpr int kItemCost = 2;          // KV tiles that an item's start and end cost, in the choice of whole rounds
+constexpr int kItemCost = 2;           // KV tiles that an item's start and end cost, in the choice of whole rounds
+constexpr int kCutCost = 8;            // KV tiles that cutting items costs (pieces, merge)
 constexpr int kTensorMinUnits = 2;    // units a program's range has at least when every item is cut
 constexpr int kMergeThreads = 256;
 constexpr int kMergeRows[2] = {8, 16};  // rows merged by one CTA, by list
@@ -52,7 +53,7 @@ __device__ __forceinline__ V block_scan(V v, V& total, V* shared) {
 }
 
 // The tensor kernel's work list: the items by descending units; whole rounds of one item per program in snake order,
-// either all of them, where that comes within 5 % and four tiles of an equal share, or as many as stay within each
+// either all of them, where that comes within 5 % and what cutting costs of an equal share, or as many as stay within each
 // program's share, the rest cut into a contiguous range of units per program that fills its share up.
 struct PlanShared {
   long long scan_l[32];
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kPlanListThreads)
       load += units > 0 ? units + kItemCost : 0;
     }
     const long long equal = (total + static_cast<long long>(items) * kItemCost) / programs;
-    if (__syncthreads_and(load <= equal + equal / 20 + 4)) {
+    if (__syncthreads_and(load <= equal + equal / 20 + kCutCost)) {
       rounds = all_rounds;
     } else {
       const long long share = mine ? program_start(total, programs, tid + 1) - program_start(total, programs, tid) : 0;

@@ -17,14 +17,6 @@
 
 namespace fgw {
 
-// A segment as the scheduler warp hands it to the other roles through a ring in shared memory: working it out takes two
-// dependent trips to L2 and some divisions, which each role doing it by itself paid at every item's start.
-struct TensorSegment {
-  ChunkSegment s;
-  int steps[2];  // KV tiles of each query tile; s.n < 0: no more work
-};
-constexpr int kSegRing = 4;
-
 template <int NB>
 struct TensorShape {
   static constexpr int kTiles = chunk_tensor_tiles(NB);
@@ -43,11 +35,10 @@ struct TensorShape {
   static constexpr int kK = kTiles * kQBytes;
   static constexpr int kV = kK + kStages * kKVBytes;
   static constexpr int kBar = kV + kStages * kKVBytes;
-  // q_full, q_empty, {k,v}_{full,empty}[S], s_full, p_half, p_full, pv_done, o_empty [2], mma_done, seg_{full,empty}[R]
-  static constexpr int kNumBars = 2 + 4 * kStages + 10 + 1 + 2 * kSegRing;
+  // q_full, q_empty, {k,v}_{full,empty}[S], s_full, p_half, p_full, pv_done, o_empty [2], mma_done
+  static constexpr int kNumBars = 2 + 4 * kStages + 10 + 1;
   static constexpr int kTmemSlot = kBar + kNumBars * 8;
-  static constexpr int kSegs = kTmemSlot + 16;
-  static constexpr int kBytes = kSegs + kSegRing * static_cast<int>(sizeof(TensorSegment)) + 1024;
+  static constexpr int kBytes = kTmemSlot + 16 + 1024;
   static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
@@ -148,9 +139,6 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
   uint64_t* pv_done = p_full + 2;   // [2]
   uint64_t* o_empty = pv_done + 2;  // [2]
   uint64_t* mma_done = o_empty + 2;
-  uint64_t* seg_full = mma_done + 1;  // [kSegRing]
-  uint64_t* seg_empty = seg_full + kSegRing;
-  TensorSegment* segs = reinterpret_cast<TensorSegment*>(smem + S::kSegs);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kTmemSlot);
 
   const int warp = threadIdx.x / 32;
@@ -172,10 +160,6 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
       mbar_init(&o_empty[t], 4);
     }
     mbar_init(mma_done, 1);
-    for (int i = 0; i < kSegRing; ++i) {
-      mbar_init(&seg_full[i], 1);
-      mbar_init(&seg_empty[i], 2 + 4 * kTiles);  // the producer, the MMA warp and the softmax warps
-    }
     fence_barrier_init();
     a.slots.errors[blockIdx.x] = make_int2(0, 0);
   }
@@ -193,20 +177,6 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
   grid_dependents_launch();
 
   if (kTiles == 2 && warp < 4) setmaxnreg_dec<S::kRegsControl>();
-  uint32_t seg_count = 0;
-  // The next segment for a converged warp, copied out of the ring; false when there is none or a wait gave up.
-  auto take_segment = [&](TensorSegment& sg) {
-    const uint32_t slot = seg_count % kSegRing;
-    if (!__all_sync(0xffffffffu, mbar_wait(&seg_full[slot], (seg_count / kSegRing) & 1, a.budget_ns))) {
-      if (lane == 0) chunk_error(a, 94);
-      return false;
-    }
-    sg = segs[slot];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&seg_empty[slot]);
-    ++seg_count;
-    return sg.s.n >= 0;
-  };
   if (warp == 0) {
     // ------------------------------------------------------------------------- TMA producer
     // Lane l issues the l-th box of a K (or V) tile: boxes x blocks of 64 values, at most 32.
@@ -228,9 +198,10 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
       }
       return ok;
     };
-    TensorSegment seg;
-    while (take_segment(seg)) {
-      const ChunkSegment& sg = seg.s;
+    TensorCursor cur;
+    cursor_init(list, cur);
+    ChunkSegment sg;
+    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, list, cur, sg)), 0)) {
       const int n = __shfl_sync(0xffffffffu, sg.n, 0);
       if (n <= 0) continue;
       if (wait_or_fail(q_empty, (qc & 1) ^ 1, 80) && lane == 0) {
@@ -317,11 +288,13 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
         asm volatile("" : "+r"(p_col), "+r"(b_lo));
       }
     };
-    TensorSegment seg;
-    while (take_segment(seg)) {
-      const int n = __shfl_sync(0xffffffffu, seg.s.n, 0);
-      const int n_a = __shfl_sync(0xffffffffu, seg.steps[0], 0);
-      const int n_b = kTiles == 2 ? __shfl_sync(0xffffffffu, seg.steps[1], 0) : 0;
+    TensorCursor cur;
+    cursor_init(list, cur);
+    ChunkSegment sg;
+    while (__shfl_sync(0xffffffffu, static_cast<int>(next_segment(a, list, cur, sg)), 0)) {
+      const int n = __shfl_sync(0xffffffffu, sg.n, 0);
+      const int n_a = __shfl_sync(0xffffffffu, tile_steps(a, sg, 0, tile_tokens), 0);
+      const int n_b = kTiles == 2 ? __shfl_sync(0xffffffffu, tile_steps(a, sg, 1, tile_tokens), 0) : 0;
       if (n <= 0) continue;
       int kst = kc % NS;
       if (wait_or_fail(q_full, qc & 1, 83) && wait_or_fail(&k_full[kst], (kc / NS) & 1, 84)) {
@@ -384,32 +357,6 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
       umma_commit_e(leader, mma_done);
       __all_sync(0xffffffffu, mbar_wait(mma_done, 0, a.budget_ns));
     }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------------------- scheduler
-    TensorCursor cur;
-    cursor_init(list, cur);
-    bool more = true;
-    for (uint32_t i = 0; more; ++i) {
-      TensorSegment seg;
-      more = next_segment(a, list, cur, seg.s);
-      seg.steps[0] = seg.steps[1] = 0;
-      if (more) {
-        seg.steps[0] = tile_steps(a, seg.s, 0, tile_tokens);
-        if (kTiles == 2) seg.steps[1] = tile_steps(a, seg.s, 1, tile_tokens);
-      } else {
-        seg.s.n = -1;
-      }
-      const uint32_t slot = i % kSegRing;
-      if (!__all_sync(0xffffffffu, mbar_wait(&seg_empty[slot], ((i / kSegRing) & 1) ^ 1, a.budget_ns))) {
-        if (lane == 0) chunk_error(a, 95);
-        break;
-      }
-      if (lane == 0) {
-        segs[slot] = seg;
-        mbar_arrive(&seg_full[slot]);
-      }
-      __syncwarp();
-    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------------- softmax / epilogue
     // Warps 4-7 own query tile A, warps 8-11 tile B; a warp reaches the TMEM lanes of its quarter (warp % 4).
@@ -430,15 +377,16 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
       }
       return ok;
     };
-    TensorSegment seg;
-    while (take_segment(seg)) {
-      const ChunkSegment& sg = seg.s;
+    TensorCursor cur;
+    cursor_init(list, cur);
+    ChunkSegment sg;
+    while (next_segment(a, list, cur, sg)) {
       const int i_tok = t * tile_tokens + row_token;  // token within the item
       const bool row_valid = row_token < tile_tokens && i_tok < sg.count;
       // rows of no token compute on whatever Q's tile holds (rows do not mix) and are never stored
       const int vis = row_valid ? seen_keys(a, sg, i_tok) : sg.limit;
-      const int n_t = t == 0 ? seg.steps[0] : seg.steps[1];
-      const int n_other = t == 0 ? 0 : seg.steps[0];
+      const int n_t = tile_steps(a, sg, t, tile_tokens);
+      const int n_other = t == 0 ? 0 : tile_steps(a, sg, 0, tile_tokens);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n_t; ++j) {
         const int tok0 = (sg.n_begin + j) * BN;
