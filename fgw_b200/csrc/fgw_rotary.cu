@@ -18,7 +18,7 @@ namespace fgw {
 
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryTokens = 4;  // at most, per CTA
-constexpr int kRotaryHeads = 2;   // heads a thread loads before it stores any
+constexpr int kRotaryHeads = 3;   // heads a thread loads together, one such batch ahead of the one it turns
 
 struct RotaryArgs {
   const void *q, *k, *v;
@@ -30,6 +30,7 @@ struct RotaryArgs {
   long long q_stride, k_stride, v_stride, out_stride;  // elements from token to token
   long long tokens, pool_pages;
   int batch, width, page, heads, kv_heads, dim, rotary, positions, per_cta;
+  int vector_angles;  // rows of cos_sin and their halves start on 16 bytes
 };
 
 struct TokenPlace {
@@ -55,29 +56,20 @@ __device__ __forceinline__ TokenPlace token_place(const RotaryArgs& a, long long
 
 // Head h of the token: queries, then keys, then values.
 template <typename T>
-struct HeadRow {
-  const T* src;
-  T* dst;     // nullptr: nothing to write
-  bool turn;  // queries and keys turn, values pass
-};
-
+__device__ __forceinline__ const T* head_source(const RotaryArgs& a, long long t, int h) {
+  if (h < a.heads) return static_cast<const T*>(a.q) + t * a.q_stride + static_cast<long long>(h) * a.dim;
+  h -= a.heads;
+  if (h < a.kv_heads) return static_cast<const T*>(a.k) + t * a.k_stride + static_cast<long long>(h) * a.dim;
+  return static_cast<const T*>(a.v) + t * a.v_stride + static_cast<long long>(h - a.kv_heads) * a.dim;
+}
+// Where it goes (nullptr: nowhere).
 template <typename T>
-__device__ __forceinline__ HeadRow<T> head_row(const RotaryArgs& a, const TokenPlace& p, long long t, int h) {
-  HeadRow<T> r;
-  if (h < a.heads) {
-    r.src = static_cast<const T*>(a.q) + t * a.q_stride + static_cast<long long>(h) * a.dim;
-    r.dst = static_cast<T*>(a.out) + t * a.out_stride + static_cast<long long>(h) * a.dim;
-    r.turn = true;
-    return r;
-  }
+__device__ __forceinline__ T* head_target(const RotaryArgs& a, const TokenPlace& p, long long t, int h) {
+  if (h < a.heads) return static_cast<T*>(a.out) + t * a.out_stride + static_cast<long long>(h) * a.dim;
+  if (p.row < 0) return nullptr;
   h -= a.heads;
   const bool key = h < a.kv_heads;
-  if (!key) h -= a.kv_heads;
-  r.src = static_cast<const T*>(key ? a.k : a.v) + t * (key ? a.k_stride : a.v_stride) + static_cast<long long>(h) * a.dim;
-  r.dst = p.row < 0 ? nullptr
-                    : static_cast<T*>(key ? a.k_cache : a.v_cache) + (p.row * a.kv_heads + h) * a.dim;
-  r.turn = key;
-  return r;
+  return static_cast<T*>(key ? a.k_cache : a.v_cache) + (p.row * a.kv_heads + (key ? h : h - a.kv_heads)) * a.dim;
 }
 
 template <typename T>
@@ -96,30 +88,35 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const Rot
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const long long first = static_cast<long long>(blockIdx.x) * a.per_cta;
   const int count = static_cast<int>(min(static_cast<long long>(a.per_cta), a.tokens - first));
-  if (warp < count) {
-    const TokenPlace p = token_place(a, first + warp, lane);
-    if (lane == 0) places[warp] = p;
-  }
-  __syncthreads();
+  auto find_places = [&]() {
+    if (warp < count) {
+      const TokenPlace p = token_place(a, first + warp, lane);
+      if (lane == 0) places[warp] = p;
+    }
+    __syncthreads();
+  };
   const int half = a.rotary / 2;
   const int all_heads = a.heads + 2 * a.kv_heads;
   if constexpr (kLayout == 2) {
+    find_places();
     const int per_head = half + a.dim - a.rotary;  // pairs, then the values that pass
     for (int k = 0; k < count; ++k) {
       const TokenPlace p = places[k];
       const float* angles = a.cos_sin + static_cast<long long>(max(p.position, 0)) * a.rotary;
       for (int i = threadIdx.x; i < all_heads * per_head; i += kRotaryThreads) {
         const int e = i % per_head;
-        const HeadRow<T> r = head_row<T>(a, p, first + k, i / per_head);
-        if (r.dst == nullptr) continue;
+        const int h = i / per_head;
+        const T* src = head_source<T>(a, first + k, h);
+        T* dst = head_target<T>(a, p, first + k, h);
+        if (dst == nullptr) continue;
         if (e >= half) {
-          r.dst[half + e] = p.position < 0 ? Tr::from_float(0.f) : r.src[half + e];
+          dst[half + e] = p.position < 0 ? Tr::from_float(0.f) : src[half + e];
           continue;
         }
-        float x = static_cast<float>(r.src[e]), y = static_cast<float>(r.src[half + e]);
-        if (r.turn) turn_pair<T>(x, y, angles[e], angles[half + e]);
-        r.dst[e] = Tr::from_float(p.position < 0 ? 0.f : x);
-        r.dst[half + e] = Tr::from_float(p.position < 0 ? 0.f : y);
+        float x = static_cast<float>(src[e]), y = static_cast<float>(src[half + e]);
+        if (h < a.heads + a.kv_heads) turn_pair<T>(x, y, angles[e], angles[half + e]);
+        dst[e] = Tr::from_float(p.position < 0 ? 0.f : x);
+        dst[half + e] = Tr::from_float(p.position < 0 ? 0.f : y);
       }
     }
     return;
@@ -129,20 +126,47 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const Rot
   const int slots = a.dim / 8 - pair_slots;
   const int groups = kRotaryThreads / slots;
   const int slot = threadIdx.x % slots, group = threadIdx.x / slots;
-  if (group >= groups) return;
   const bool two = slot < pair_slots;
   const int at0 = two ? slot : slot + pair_slots;  // chunk within the head
   const int at1 = at0 + pair_slots;                // its partner (two)
+  // The rows' values do not depend on their place, so a batch of heads is loaded while the places are found, or the
+  // batch before is turned and stored.
+  const int batches = (all_heads + groups * kRotaryHeads - 1) / (groups * kRotaryHeads);
+  uint4 x[kRotaryHeads], y[kRotaryHeads];
+  auto load = [&](int k, int batch) {
+#pragma unroll
+    for (int u = 0; u < kRotaryHeads; ++u) {
+      const int h = group + (batch * kRotaryHeads + u) * groups;
+      if (group >= groups || h >= all_heads) continue;
+      const uint4* src = reinterpret_cast<const uint4*>(head_source<T>(a, first + k, h));
+      x[u] = src[at0];
+      if (two) y[u] = src[at1];
+    }
+  };
+  load(0, 0);
+  find_places();
+  if (group >= groups) return;
   for (int k = 0; k < count; ++k) {
     const TokenPlace p = places[k];
-    float c[8], s[8];
+    alignas(16) float c[8], s[8];
     if (p.position >= 0) {
       const float* angles = a.cos_sin + static_cast<long long>(p.position) * a.rotary;
-      if (two) {
+      if (two && a.vector_angles) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          *reinterpret_cast<float4*>(&c[i]) = *reinterpret_cast<const float4*>(&angles[slot * 8 + i]);
+          *reinterpret_cast<float4*>(&s[i]) = *reinterpret_cast<const float4*>(&angles[half + slot * 8 + i]);
+        }
+      } else if (two) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           c[i] = angles[slot * 8 + i];
           s[i] = angles[half + slot * 8 + i];
+        }
+      } else if (kLayout == 0 && a.vector_angles) {
+        if (slot * 4 < half) {
+          *reinterpret_cast<float4*>(&c[0]) = *reinterpret_cast<const float4*>(&angles[slot * 4]);
+          *reinterpret_cast<float4*>(&s[0]) = *reinterpret_cast<const float4*>(&angles[half + slot * 4]);
         }
       } else if (kLayout == 0) {
 #pragma unroll
@@ -153,27 +177,30 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const Rot
         }
       }
     }
-    for (int h0 = group; h0 < all_heads; h0 += groups * kRotaryHeads) {
-      uint4 x[kRotaryHeads], y[kRotaryHeads];
-      HeadRow<T> rows[kRotaryHeads];
+    for (int batch = 0; batch < batches; ++batch) {
+      uint4 xt[kRotaryHeads], yt[kRotaryHeads];
 #pragma unroll
       for (int u = 0; u < kRotaryHeads; ++u) {
-        const int h = h0 + u * groups;
-        rows[u].dst = nullptr;
-        if (h >= all_heads) continue;
-        rows[u] = head_row<T>(a, p, first + k, h);
-        if (rows[u].dst == nullptr) continue;
-        x[u] = reinterpret_cast<const uint4*>(rows[u].src)[at0];
-        if (two) y[u] = reinterpret_cast<const uint4*>(rows[u].src)[at1];
+        xt[u] = x[u];
+        yt[u] = y[u];
+      }
+      if (batch + 1 < batches) {
+        load(k, batch + 1);
+      } else if (k + 1 < count) {
+        load(k + 1, 0);
       }
 #pragma unroll
       for (int u = 0; u < kRotaryHeads; ++u) {
-        if (rows[u].dst == nullptr) continue;
-        uint32_t* xw = reinterpret_cast<uint32_t*>(&x[u]);
-        uint32_t* yw = reinterpret_cast<uint32_t*>(&y[u]);
+        const int h = group + (batch * kRotaryHeads + u) * groups;
+        if (h >= all_heads) continue;
+        uint4* dst = reinterpret_cast<uint4*>(head_target<T>(a, p, first + k, h));
+        if (dst == nullptr) continue;
+        const bool turn = h < a.heads + a.kv_heads;
+        uint32_t* xw = reinterpret_cast<uint32_t*>(&xt[u]);
+        uint32_t* yw = reinterpret_cast<uint32_t*>(&yt[u]);
         if (p.position < 0) {
-          x[u] = y[u] = make_uint4(0, 0, 0, 0);
-        } else if (rows[u].turn && two) {
+          xt[u] = yt[u] = make_uint4(0, 0, 0, 0);
+        } else if (turn && two) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float2 xs = Tr::unpack2(xw[i]), ys = Tr::unpack2(yw[i]);
@@ -182,7 +209,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const Rot
             xw[i] = Tr::pack2(xs.x, xs.y);
             yw[i] = Tr::pack2(ys.x, ys.y);
           }
-        } else if (rows[u].turn && kLayout == 0) {
+        } else if (turn && kLayout == 0) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (slot * 4 + i >= half) continue;
@@ -191,8 +218,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(const Rot
             xw[i] = Tr::pack2(xs.x, xs.y);
           }
         }
-        reinterpret_cast<uint4*>(rows[u].dst)[at0] = x[u];
-        if (two) reinterpret_cast<uint4*>(rows[u].dst)[at1] = y[u];
+        dst[at0] = xt[u];
+        if (two) dst[at1] = yt[u];
       }
     }
   }
@@ -268,6 +295,7 @@ cudaError_t launch_rotary(const fgw_rotary_params& p, int sm_count, cudaStream_t
   a.dim = p.head_dim;
   a.rotary = p.rotary_dim;
   a.positions = p.positions;
+  a.vector_angles = p.rotary_dim % 8 == 0 && reinterpret_cast<uintptr_t>(p.cos_sin) % 16 == 0;
   // one token per CTA until the card is full of CTAs
   a.per_cta = static_cast<int>(std::max(1ll, std::min<long long>(kRotaryTokens, p.tokens / (8ll * sm_count))));
   const unsigned grid = static_cast<unsigned>((p.tokens + a.per_cta - 1) / a.per_cta);
