@@ -220,11 +220,6 @@ def struct_format(cls):
     return "@" + "".join(_FORMATS[kind] for _, kind in cls._fields_)
 
 
-def address_of(data):
-    """Address of a bytes object's contents (valid while the caller holds it)."""
-    return ctypes.cast(data, ctypes.c_void_p).value
-
-
 _LIB = None
 
 

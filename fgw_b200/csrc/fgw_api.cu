@@ -521,7 +521,7 @@ static int page_op(const fgw_page_params* params, int op, void* workspace, size_
   int device = 0, sms = 0;
   st = current_device(&device, &sms);
   if (st != FGW_OK) return st;
-  const cudaError_t err = launch_page_op(*params, op, workspace, sms, static_cast<cudaStream_t>(stream));
+  const cudaError_t err = launch_page_op(*params, op, workspace, sms, device, static_cast<cudaStream_t>(stream));
   return err == cudaSuccess ? FGW_OK : FGW_ERR_CUDA;
 }
 

@@ -48,27 +48,6 @@ struct ChunkList {
   int max_rows;
 };
 
-// Division of 0 <= n < 2^31 by a fixed positive number with a multiplication and shifts (Granlund and Montgomery, "Division
-// by invariant integers using multiplication", 1994): m = floor(2^32 (2^l - d) / d) + 1 with 2^l >= d, q = (t + (n - t) / 2)
-// / 2^(l - 1) with t = floor(m n / 2^32). A division by a variable takes some 150 cycles, and the kernels' starts are
-// chains of them.
-struct FastDiv {
-  uint32_t mul, shift, one;  // one: the divisor is 1
-  int by;
-  FastDiv() = default;
-  explicit FastDiv(int d) : by(d) {
-    uint32_t l = 0;
-    while (l < 31 && (1u << l) < static_cast<uint32_t>(d)) ++l;
-    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - d)) / d + 1);
-    shift = l > 0 ? l - 1 : 0;
-    one = l == 0;
-  }
-  __device__ __forceinline__ int quotient(int n) const {
-    const uint32_t u = static_cast<uint32_t>(n), t = __umulhi(mul, u);
-    return one ? n : static_cast<int>((t + ((u - t) >> 1)) >> shift);
-  }
-};
-
 struct ChunkArgs {
   void* out;
   const int32_t* table;

@@ -422,12 +422,12 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
         }
         const float mx = max3(mq0, mq1, fmaxf(mq2, mq3)) * a.scale_log2;  // scale > 0; -inf stays -inf
         // The maximum moves only when it grows by more than 2^8 (P then stays below 2^8, far inside both types' range),
-        // so O is rarely rescaled.
-        float m_new = j == 0 ? mx : m;
+        // so O is rarely rescaled. Each row decides for itself: what other rows of the warp hold leaves its bits alone.
+        const bool grow = j > 0 && mx > m + 8.0f;
+        const float m_new = j == 0 || grow ? mx : m;
         float alpha = 1.f;
-        if (__any_sync(0xffffffffu, j > 0 && mx > m + 8.0f)) {
-          m_new = fmaxf(m, mx);
-          alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - m_new);
+        if (__any_sync(0xffffffffu, grow)) {
+          if (grow) alpha = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
           if (ok) {
             // the commit that published S_t(j) also covers PV_t(j - 1): O_t is stable
             for (int cb = 0; cb < D / 16; ++cb) {

@@ -113,7 +113,8 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_coun
 enum PageOp { kPageFork = 0, kPageCompact = 1, kPageCopy = 2 };
 int page_validate(const fgw_page_params& p, int op);
 size_t page_workspace_bytes(const fgw_page_params& p, int op);
-cudaError_t launch_page_op(const fgw_page_params& p, int op, void* workspace, int sm_count, cudaStream_t stream);
+cudaError_t launch_page_op(const fgw_page_params& p, int op, void* workspace, int sm_count, int device,
+                           cudaStream_t stream);
 cudaError_t launch_plan(const LaunchDesc& d);
 // fused_merge (with write_partials): the CTA completing a group's split set merges it into the output.
 cudaError_t launch_decode(const LaunchDesc& d, bool write_partials, bool fused_merge);

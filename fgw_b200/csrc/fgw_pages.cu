@@ -5,27 +5,33 @@
 // its row, and a page that no row holds is free. So there are no counts or free lists that could disagree with the
 // table, and a row is freed by giving it no parent.
 //
-// One cluster of eight CTAs does the bookkeeping (page_plan_kernel): it marks the held pages in a bitmap, ranks the
-// free pages by a prefix sum over the bitmap, hands them out in (row, column) order and leaves a list of the pages to
-// copy. All of it is integer work in a fixed order (atomics only where the order cannot show: OR, MIN, ADD of counts),
-// so results do not depend on timing. It is bound by latency: a chain of cluster barriers, each around one or two
-// round trips to L2. page_copy_kernel then moves the bytes, bound by HBM.
+// page_plan_kernel does the bookkeeping: it marks the held pages in a bitmap, ranks the free pages by a prefix sum over
+// the bitmap, hands them out in (row, column) order and leaves a list of the pages to copy. All of it is integer work in
+// a fixed order (atomics only where the order cannot show: OR, MIN, ADD of counts), so results do not depend on timing.
+// It is bound by latency: a chain of barriers, each around one or two round trips to L2. Tables of up to 32K entries over
+// up to 128K pages are one CTA's work with the bitmap and the row arrays in shared memory; larger ones go to a cluster
+// of eight CTAs over global memory. page_copy_kernel then moves the bytes, bound by HBM; it is launched beside the plan
+// and waits for it.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fgw_common.cuh"
 #include "fgw_kernels.h"
+#include "fgw_ragged.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace fgw {
 
 constexpr int kPlanCtas = 8;       // one portable cluster
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 1024;
+constexpr int kSmallPages = 1 << 17, kSmallRows = 4096, kSmallEntries = 1 << 15;  // one CTA's share
+constexpr int kPlanLoads = 4;
 constexpr int kBlockWords = 32;    // bitmap words ranked together by one warp (1024 pages)
 constexpr int kCopyThreads = 256;
-constexpr int kCopyUnroll = 4;
+constexpr int kCopyUnroll = 8;  // 32 KB of a page per step: 257 us against 263 with 16 KB (1.47 GB moved)
 constexpr int kPoolsPerLaunch = 224;  // pool pointers passed by value in one copy launch
 
 struct PageCopy {
@@ -38,9 +44,10 @@ struct PageWs {
   int32_t* totals;   // [0] copies, [1] needed pages, [2] free pages, [3] moved pages
   uint32_t* used;    // bitmap of the held pages
   int32_t* blocks;   // free pages before each block of 1024 pages, exclusive
-  int32_t* list;     // fork: free pages in order; compact: holes, then new ids of the moved pages
+  int32_t* list;     // fork: free pages in order; compact: holes, moved pages (last first), then new ids by page
   int32_t* first;    // [batch] first row with this parent
   int32_t* need;     // [batch + 1] new pages of each row, then their exclusive prefix
+  int4* rows;        // [batch] what each row becomes: {parent, entries kept, entries wanted, entries held}
 };
 
 struct PageArgs {
@@ -53,6 +60,7 @@ struct PageArgs {
   int32_t* status;
   PageWs ws;
   int batch, width, page, pages, words, blocks;
+  FastDiv by_width;
 };
 
 static size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -72,9 +80,10 @@ static size_t carve_pages(const fgw_page_params& p, void* base, PageWs* ws) {
   w.copies = reinterpret_cast<PageCopy*>(take(copies * sizeof(PageCopy)));
   w.used = reinterpret_cast<uint32_t*>(take(blocks * kBlockWords * 4));
   w.blocks = reinterpret_cast<int32_t*>(take((blocks + 1) * 4));
-  w.list = reinterpret_cast<int32_t*>(take(2 * static_cast<size_t>(p.num_pages) * 4));
+  w.list = reinterpret_cast<int32_t*>(take(3 * static_cast<size_t>(p.num_pages) * 4));
   w.first = reinterpret_cast<int32_t*>(take(static_cast<size_t>(p.batch) * 4));
   w.need = reinterpret_cast<int32_t*>(take((static_cast<size_t>(p.batch) + 1) * 4));
+  w.rows = reinterpret_cast<int4*>(take(static_cast<size_t>(p.batch) * 16));
   if (ws != nullptr) *ws = w;
   return static_cast<size_t>(at - static_cast<uint8_t*>(base));
 }
@@ -105,21 +114,14 @@ __device__ __forceinline__ ForkRow fork_row(const PageArgs& a, int i) {
   return r;
 }
 
-__device__ __forceinline__ void mark_row(const PageArgs& a, int row, int held, int lane, int lanes) {
-  const int32_t* entries = a.table + static_cast<long long>(row) * a.width;
-  for (int w = lane; w < held; w += lanes) {
-    const int id = entries[w];
-    if (id >= 0 && id < a.pages) atomicOr(&a.ws.used[id >> 5], 1u << (id & 31));
-  }
-}
-
 // Exclusive prefix sum of x[0, n) in place by one CTA; returns the total to every thread.
-__device__ int cta_exclusive_scan(int32_t* x, int n, int* shared) {
+template <typename Load>
+__device__ int cta_exclusive_scan(int32_t* x, int n, int* shared, Load load) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int carry = 0;
   for (int base = 0; base < n; base += blockDim.x) {
     const int i = base + threadIdx.x;
-    const int v = i < n ? x[i] : 0;
+    const int v = i < n ? load(&x[i]) : 0;
     int sum = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -140,12 +142,45 @@ __device__ int cta_exclusive_scan(int32_t* x, int n, int* shared) {
   return carry;
 }
 
-template <bool kFork>
-__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) page_plan_kernel(const PageArgs a) {
-  cg::cluster_group cluster = cg::this_cluster();
-  __shared__ int shared[32];
+// Scratch of the one-CTA form in shared memory.
+struct SmallWs {
+  int32_t totals[4];
+  uint32_t used[kSmallPages / 32];
+  int32_t blocks[kSmallPages / (32 * kBlockWords) + 1];
+  int32_t first[kSmallRows];
+  int32_t need[kSmallRows + 1];
+  alignas(16) int4 rows[kSmallRows];
+};
+
+template <bool kFork, int kCtas>
+__device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
+  extern __shared__ uint8_t plan_smem[];
+  if constexpr (kCtas == 1) {
+    SmallWs& small = *reinterpret_cast<SmallWs*>(plan_smem);
+    a.ws.used = small.used;
+    a.ws.blocks = small.blocks;
+    a.ws.first = small.first;
+    a.ws.need = small.need;
+    a.ws.rows = small.rows;
+  }
+  int32_t* totals = kCtas == 1 ? reinterpret_cast<SmallWs*>(plan_smem)->totals : a.ws.totals;
+  auto sync = [&]() {
+    if constexpr (kCtas == 1) {
+      __syncthreads();
+    } else {
+      cg::this_cluster().sync();
+    }
+  };
+  // what other threads have written since the last barrier, past this SM's L1
+  auto fresh = [&](const auto* x) {
+    if constexpr (kCtas == 1) {
+      return *const_cast<const volatile std::remove_reference_t<decltype(*x)>*>(x);
+    } else {
+      return __ldcg(x);
+    }
+  };
   const int tid = blockIdx.x * kPlanThreads + threadIdx.x;
-  constexpr int kThreads = kPlanCtas * kPlanThreads;
+  constexpr int kThreads = kCtas * kPlanThreads;
   const int lane = threadIdx.x & 31;
   const int warp = tid >> 5;
   constexpr int kWarps = kThreads / 32;
@@ -158,56 +193,79 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     if (first_page + 32 > a.pages) bits = first_page >= a.pages ? 0xffffffffu : 0xffffffffu << (a.pages & 31);
     a.ws.used[w] = bits;
   }
-  if (kFork) {
-    for (int i = tid; i < a.batch; i += kThreads) a.ws.first[i] = a.batch;
-  }
-  if (tid < 4) a.ws.totals[tid] = 0;
-  cluster.sync();
-  if (kFork) {
-    for (int i = tid; i < a.batch; i += kThreads) {
-      const int parent = a.parents[i];
-      if (parent >= 0 && parent < a.batch) atomicMin(&a.ws.first[parent], i);
-    }
-    cluster.sync();
-  }
-  // The held pages; of the rows with one parent only the first marks.
-  for (int i = warp; i < a.batch; i += kWarps) {
+  if (tid < 4) totals[tid] = 0;
+  for (int i = tid; i < a.batch; i += kThreads) {
     if (kFork) {
+      a.ws.first[i] = a.batch;
       const ForkRow r = fork_row(a, i);
-      const bool is_first = r.parent >= 0 && __ldcg(&a.ws.first[r.parent]) == i;
-      if (is_first) mark_row(a, r.parent, r.held, lane, 32);
-      const int copy = r.parent >= 0 && !is_first && r.len > r.full * a.page;
-      if (lane == 0) a.ws.need[i] = copy + r.want - r.held;
+      a.ws.rows[i] = make_int4(r.parent, r.held, r.want, r.held);
     } else {
       const int len = clamped_len(a, a.lens[i]);
-      mark_row(a, i, len / a.page + (len % a.page != 0), lane, 32);
+      a.ws.rows[i] = make_int4(i, 0, 0, len / a.page + (len % a.page != 0));
     }
   }
-  cluster.sync();
+  sync();
+  if (kFork) {
+    for (int i = tid; i < a.batch; i += kThreads) {
+      const int parent = fresh(&a.ws.rows[i].x);
+      if (parent >= 0) atomicMin(&a.ws.first[parent], i);
+    }
+    sync();
+  }
+  // The held pages; of the rows with one parent only the first marks. Table entries are taken flat, four loads of a
+  // thread at a time.
+  const int entries = a.batch * a.width;
+  for (int base = tid; base < entries; base += kThreads * kPlanLoads) {
+    int ids[kPlanLoads];
+#pragma unroll
+    for (int u = 0; u < kPlanLoads; ++u) {
+      ids[u] = -1;
+      const long long at = base + static_cast<long long>(u) * kThreads;
+      if (at >= entries) continue;
+      const int i = a.by_width.quotient(static_cast<int>(at)), w = static_cast<int>(at) - i * a.width;
+      const int parent = fresh(&a.ws.rows[i].x), held = fresh(&a.ws.rows[i].w);
+      if (w >= held || (kFork && fresh(&a.ws.first[parent]) != i)) continue;  // held is 0 without a parent
+      ids[u] = a.table[static_cast<long long>(parent) * a.width + w];
+    }
+#pragma unroll
+    for (int u = 0; u < kPlanLoads; ++u) {
+      if (ids[u] >= 0 && ids[u] < a.pages) atomicOr(&a.ws.used[ids[u] >> 5], 1u << (ids[u] & 31));
+    }
+  }
+  if (kFork) {
+    for (int i = tid; i < a.batch; i += kThreads) {
+      const ForkRow r = fork_row(a, i);
+      const bool copies = r.parent >= 0 && r.len > r.full * a.page && fresh(&a.ws.first[r.parent]) != i;
+      a.ws.need[i] = (copies ? 1 : 0) + r.want - r.held;
+      if (copies) a.ws.rows[i].y = r.full;
+    }
+  }
+  sync();
   for (int b = warp; b < a.blocks; b += kWarps) {
-    const int free_here = 32 - __popc(__ldcg(&a.ws.used[b * kBlockWords + lane]));
+    const int free_here = 32 - __popc(fresh(&a.ws.used[b * kBlockWords + lane]));
     const int sum = __reduce_add_sync(0xffffffffu, free_here);
     if (lane == 0) a.ws.blocks[b] = sum;
   }
-  cluster.sync();
+  sync();
   if (blockIdx.x == 0) {
-    const int free_pages = cta_exclusive_scan(a.ws.blocks, a.blocks, shared);
-    if (threadIdx.x == 0) a.ws.totals[2] = free_pages;
-  } else if (kFork && blockIdx.x == 1) {
-    const int needed = cta_exclusive_scan(a.ws.need, a.batch, shared);
-    if (threadIdx.x == 0) a.ws.totals[1] = needed;
+    const int free_pages = cta_exclusive_scan(a.ws.blocks, a.blocks, shared, fresh);
+    if (threadIdx.x == 0) totals[2] = free_pages;
   }
-  cluster.sync();
-  const int free_pages = __ldcg(&a.ws.totals[2]);
+  if (kFork && blockIdx.x == (kCtas > 1 ? 1 : 0)) {
+    const int needed = cta_exclusive_scan(a.ws.need, a.batch, shared, fresh);
+    if (threadIdx.x == 0) totals[1] = needed;
+  }
+  sync();
+  const int free_pages = fresh(&totals[2]);
   const int live = a.pages - free_pages;
-  const int needed = kFork ? __ldcg(&a.ws.totals[1]) : 0;
+  const int needed = kFork ? fresh(&totals[1]) : 0;
   // Fork: the first `needed` free pages in order. Compact: the free pages below `live` (list[rank]) and the held
   // pages from `live` on, which are the last in the order of held pages (list[pages + live - 1 - rank]).
   for (int b = warp; b < a.blocks; b += kWarps) {
-    int rank = __ldcg(&a.ws.blocks[b]);
+    int rank = fresh(&a.ws.blocks[b]);
     if (kFork && rank >= needed) continue;
     const int w = b * kBlockWords + lane;
-    const uint32_t used = __ldcg(&a.ws.used[w]);
+    const uint32_t used = fresh(&a.ws.used[w]);
     const int free_here = 32 - __popc(used);
     int sum = free_here;
 #pragma unroll
@@ -216,6 +274,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       if (lane >= d) sum += up;
     }
     rank += sum - free_here;
+    int moves = 0;
     for (int bit = 0; bit < 32; ++bit) {
       const int id = w * 32 + bit;
       if ((used >> bit & 1) == 0) {
@@ -224,91 +283,104 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
       } else if (!kFork && id >= live && id < a.pages) {
         const int held_rank = id - rank;  // held pages before this one
         a.ws.list[a.pages + live - 1 - held_rank] = id;
-        atomicAdd(&a.ws.totals[3], 1);
+        ++moves;
       }
     }
+    if (!kFork) {
+      moves = __reduce_add_sync(0xffffffffu, moves);
+      if (lane == 0 && moves > 0) atomicAdd(&totals[3], moves);
+    }
   }
-  cluster.sync();
+  sync();
+  const bool fits = needed <= free_pages;  // else the state stays as it was
+  const int moved = kFork ? 0 : fresh(&totals[3]);
+  int32_t* new_id = a.ws.list + 2ll * a.pages;
   if (kFork) {
-    const bool fits = needed <= free_pages;
-    for (int i = warp; i < a.batch; i += kWarps) {
+    for (int i = tid; i < a.batch; i += kThreads) {
       const ForkRow r = fork_row(a, i);
-      int32_t* out = a.table_out + static_cast<long long>(i) * a.width;
-      if (!fits) {  // the state stays as it was
-        const int32_t* in = a.table + static_cast<long long>(i) * a.width;
-        for (int w = lane; w < a.width; w += 32) out[w] = in[w];
-        if (lane == 0) a.lens_out[i] = a.lens[i];
-        continue;
-      }
-      const int32_t* in = a.table + static_cast<long long>(max(r.parent, 0)) * a.width;
-      const bool copies = r.parent >= 0 && r.len > r.full * a.page && __ldcg(&a.ws.first[r.parent]) != i;
-      const int kept = copies ? r.full : r.held;  // entries taken over as they are
-      const int base = __ldcg(&a.ws.need[i]);
-      for (int w = lane; w < a.width; w += 32) {
-        out[w] = w < kept ? in[w] : (w < r.want ? __ldcg(&a.ws.list[base + w - kept]) : -1);
-      }
-      if (lane == 0) {
-        a.lens_out[i] = r.len;
-        if (copies) {
-          const int src = in[r.full];
-          const int at = atomicAdd(&a.ws.totals[0], 1);
-          a.ws.copies[at] = {src, __ldcg(&a.ws.list[base]), src >= 0 && src < a.pages ? r.len - r.full * a.page : 0};
-        }
-      }
+      a.lens_out[i] = fits ? r.len : a.lens[i];
+      if (!fits || r.parent < 0 || r.len <= r.full * a.page || fresh(&a.ws.first[r.parent]) == i) continue;
+      const int src = a.table[static_cast<long long>(r.parent) * a.width + r.full];
+      const int dst = __ldcg(&a.ws.list[fresh(&a.ws.need[i])]);
+      const int at = atomicAdd(&totals[0], 1);
+      a.ws.copies[at] = {src, dst, src >= 0 && src < a.pages ? r.len - r.full * a.page : 0};
     }
     if (tid == 0) {
       a.status[0] = needed;
       a.status[1] = free_pages;
     }
   } else {
-    const int moved = __ldcg(&a.ws.totals[3]);
     const int32_t* movers = a.ws.list + a.pages;  // [k] = the (moved - 1 - k)-th moved page
     for (int k = tid; k < moved; k += kThreads) {
-      const int src = __ldcg(&movers[moved - 1 - k]);
-      a.ws.copies[k] = {src, __ldcg(&a.ws.list[k]), a.page};
+      const int src = __ldcg(&movers[moved - 1 - k]), dst = __ldcg(&a.ws.list[k]);
+      a.ws.copies[k] = {src, dst, a.page};
+      new_id[src] = dst;
     }
     if (tid == 0) {
       a.ws.totals[0] = moved;
       a.status[0] = live;
       a.status[1] = moved;
     }
-    cluster.sync();
-    for (int i = warp; i < a.batch; i += kWarps) {
-      const int len = clamped_len(a, a.lens[i]);
-      const int held = len / a.page + (len % a.page != 0);
-      const int32_t* in = a.table + static_cast<long long>(i) * a.width;
-      int32_t* out = a.table_out + static_cast<long long>(i) * a.width;
-      for (int w = lane; w < a.width; w += 32) {
-        int id = w < held ? in[w] : -1;
-        if (id >= live && id < a.pages) {
-          // the moved pages are in order in copies[].src: the k-th goes to the k-th hole
-          int lo = 0, hi = moved - 1;
-          while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (__ldcg(&a.ws.copies[mid].src) < id) {
-              lo = mid + 1;
-            } else {
-              hi = mid;
-            }
-          }
-          id = __ldcg(&a.ws.copies[lo].dst);
-        }
-        out[w] = id;
+    sync();
+  }
+  for (int base = tid; base < entries; base += kThreads * kPlanLoads) {
+    int ids[kPlanLoads];
+#pragma unroll
+    for (int u = 0; u < kPlanLoads; ++u) {
+      ids[u] = -1;
+      const long long at = base + static_cast<long long>(u) * kThreads;
+      if (at >= entries) continue;
+      const int i = a.by_width.quotient(static_cast<int>(at)), w = static_cast<int>(at) - i * a.width;
+      if (kFork && !fits) {
+        ids[u] = a.table[at];
+        continue;
+      }
+      const int parent = fresh(&a.ws.rows[i].x);
+      const int kept = kFork ? fresh(&a.ws.rows[i].y) : fresh(&a.ws.rows[i].w);  // taken over as they are
+      if (w < kept) {
+        ids[u] = a.table[static_cast<long long>(parent) * a.width + w];
+      } else if (kFork && w < fresh(&a.ws.rows[i].z)) {
+        ids[u] = __ldcg(&a.ws.list[fresh(&a.ws.need[i]) + w - kept]);
       }
     }
+#pragma unroll
+    for (int u = 0; u < kPlanLoads; ++u) {
+      const long long at = base + static_cast<long long>(u) * kThreads;
+      if (at >= entries) continue;
+      if (!kFork && ids[u] >= live && ids[u] < a.pages) ids[u] = __ldcg(&new_id[ids[u]]);
+      a.table_out[at] = ids[u];
+    }
   }
+  if (kFork && kCtas == 1) {
+    sync();
+    if (tid == 0) a.ws.totals[0] = totals[0];
+  }
+}
+
+template <bool kFork>
+__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) page_plan_kernel(const PageArgs a) {
+  __shared__ int shared[32];
+  grid_dependents_launch();
+  page_plan<kFork, kPlanCtas>(a, shared);
+}
+template <bool kFork>
+__global__ void __launch_bounds__(kPlanThreads) page_plan_small_kernel(const PageArgs a) {
+  __shared__ int shared[32];
+  grid_dependents_launch();
+  page_plan<kFork, 1>(a, shared);
 }
 
 struct PoolList {
   void* at[kPoolsPerLaunch];
 };
 
-// Copies the listed pages' rows in every pool, 16 KB of one page at a time. Sources and destinations are distinct
+// Copies the listed pages' rows in every pool, 32 KB of one page at a time. Sources and destinations are distinct
 // pages (held and free ones), so the order of the copies does not matter.
 __global__ void __launch_bounds__(kCopyThreads)
     page_copy_kernel(const __grid_constant__ PoolList pools, int pool_count, const PageCopy* list,
                      const int32_t* list_count, long long page_units, long long row_units) {
   constexpr int kChunk = kCopyThreads * kCopyUnroll;
+  grid_dependency_wait();  // the plan's list
   const long long chunks = (page_units + kChunk - 1) / kChunk;
   const long long units = static_cast<long long>(*list_count) * pool_count * chunks;
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
@@ -334,7 +406,7 @@ __global__ void __launch_bounds__(kCopyThreads)
 }
 
 // The caller's page lists as a copy list: entries with a page outside the pool are skipped.
-__global__ void page_list_kernel(const int32_t* src, const int32_t* dst, int n, int pages, int page, PageCopy* list,
+__global__ void __launch_bounds__(256) page_list_kernel(const int32_t* src, const int32_t* dst, int n, int pages, int page, PageCopy* list,
                                  int32_t* count) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i == 0) *count = n;
@@ -350,12 +422,34 @@ static cudaError_t launch_copies(const fgw_page_params& p, const PageCopy* list,
     const int n = std::min(kPoolsPerLaunch, p.pool_count - at);
     PoolList pools;
     for (int i = 0; i < kPoolsPerLaunch; ++i) pools.at[i] = i < n ? p.pools[at + i] : nullptr;
-    page_copy_kernel<<<8 * sm_count, kCopyThreads, 0, stream>>>(pools, n, list, count, row_units * p.page_size,
-                                                                row_units);
-    const cudaError_t err = cudaGetLastError();
+    // the first waits for the plan only where it runs; the others follow it in stream order
+    cudaError_t err;
+    if (at == 0) {
+      err = launch_after_plan(page_copy_kernel, 8 * sm_count, kCopyThreads, 0, stream, pools, n, list, count,
+                              row_units * p.page_size, row_units);
+    } else {
+      page_copy_kernel<<<8 * sm_count, kCopyThreads, 0, stream>>>(pools, n, list, count, row_units * p.page_size,
+                                                                  row_units);
+      err = cudaGetLastError();
+    }
     if (err != cudaSuccess) return err;
   }
   return cudaSuccess;
+}
+
+template <bool kFork>
+static cudaError_t launch_plan_op(const PageArgs& a, int device, cudaStream_t stream) {
+  const bool small = a.pages <= kSmallPages && a.batch <= kSmallRows &&
+                     static_cast<long long>(a.batch) * a.width <= kSmallEntries;
+  if (!small) {
+    page_plan_kernel<kFork><<<kPlanCtas, kPlanThreads, 0, stream>>>(a);
+    return cudaGetLastError();
+  }
+  auto kernel = page_plan_small_kernel<kFork>;
+  const cudaError_t err = prepare_kernel(reinterpret_cast<const void*>(kernel), sizeof(SmallWs), device, nullptr);
+  if (err != cudaSuccess) return err;
+  kernel<<<1, kPlanThreads, sizeof(SmallWs), stream>>>(a);
+  return cudaGetLastError();
 }
 
 int page_validate(const fgw_page_params& p, int op) {
@@ -395,7 +489,8 @@ size_t page_workspace_bytes(const fgw_page_params& p, int op) {
   return carve_pages(p, nullptr, nullptr);
 }
 
-cudaError_t launch_page_op(const fgw_page_params& p, int op, void* workspace, int sm_count, cudaStream_t stream) {
+cudaError_t launch_page_op(const fgw_page_params& p, int op, void* workspace, int sm_count, int device,
+                           cudaStream_t stream) {
   if (op == kPageCopy) {
     if (p.copy_count == 0 || p.pool_count == 0) return cudaSuccess;
     int32_t* count = static_cast<int32_t*>(workspace);
@@ -418,14 +513,10 @@ cudaError_t launch_page_op(const fgw_page_params& p, int op, void* workspace, in
   a.width = p.table_width;
   a.page = p.page_size;
   a.pages = p.num_pages;
+  a.by_width = FastDiv(p.table_width);
   a.words = (p.num_pages + 31) / 32;
   a.blocks = (a.words + kBlockWords - 1) / kBlockWords;
-  if (op == kPageFork) {
-    page_plan_kernel<true><<<kPlanCtas, kPlanThreads, 0, stream>>>(a);
-  } else {
-    page_plan_kernel<false><<<kPlanCtas, kPlanThreads, 0, stream>>>(a);
-  }
-  const cudaError_t err = cudaGetLastError();
+  const cudaError_t err = op == kPageFork ? launch_plan_op<true>(a, device, stream) : launch_plan_op<false>(a, device, stream);
   return err != cudaSuccess ? err : launch_copies(p, a.ws.copies, a.ws.totals, sm_count, stream);
 }
 

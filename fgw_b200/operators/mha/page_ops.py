@@ -7,6 +7,7 @@ on the host, and give new tables, so that a step in flight can go on reading the
 
 ``pools`` are the K and V caches of every layer, tensors of one shape [num_pages * page_size, ...] and type.
 """
+import array
 import operator
 import struct
 
@@ -69,8 +70,8 @@ def _run(call, size_key, pools, page_size, device, *pointers):
     width, copies); ``pointers`` the tables' and lists' data pointers in the order of ``fgw_page_params``."""
     at, row_bytes, pages, _ = pools
     batch, width, copies = size_key
-    addresses = struct.pack(f"{len(at)}Q", *at)
-    params = _PACK(_native.address_of(addresses), *pointers, row_bytes, len(at), batch, width, page_size, pages, copies,
+    addresses = array.array("Q", at)  # host memory that outlives the call
+    params = _PACK(addresses.buffer_info()[0], *pointers, row_bytes, len(at), batch, width, page_size, pages, copies,
                    0, 0)
     nbytes = _native.page_workspace_bytes(batch, pages, copies)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)

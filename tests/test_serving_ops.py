@@ -115,6 +115,102 @@ def test_chunk_attention(case, dtype):
     check_attention(got, q, k, v, table, lens, cu, page, causal, dim ** -0.5)
 
 
+def torch_attention(q, k, v, table, lens, cu, page, causal):
+    """(out, spread) as oracle/serving.py gives them, in 64 bits with torch on the GPU, for the larger shapes."""
+    q, k, v = q.double(), k.double(), v.double()
+    out, spread = torch.zeros_like(q), torch.zeros_like(q)
+    group = q.shape[1] // k.shape[1]
+    for b, length in enumerate(lens.tolist()):
+        first, n = int(cu[b]), int(cu[b + 1] - cu[b])
+        at = torch.arange(length, device="cuda")
+        rows = torch.as_tensor(table[b], device="cuda").long()[at // page] * page + at % page
+        seen = (length - n + 1 + torch.arange(n, device="cuda")) if causal else torch.full((n,), length, device="cuda")
+        hidden = at >= seen[:, None]
+        for h in range(q.shape[1]):
+            keys, values = k[rows, h // group], v[rows, h // group]
+            s = (q[first:first + n, h] @ keys.T * q.shape[2] ** -0.5).masked_fill(hidden, -math.inf)
+            p = torch.softmax(s, -1).nan_to_num(0.0)  # rows without keys
+            out[first:first + n, h], spread[first:first + n, h] = p @ values, p @ values.abs()
+    return out, spread
+
+
+# batches with several items per CTA: chunks that need one tile and two, requests of both kernels, items cut and whole
+LARGE = [
+    # (name, new tokens, held, heads, kv heads, dim, page, causal)
+    ("prompts", [70, 300, 1, 128, 257, 1000, 20, 129, 511, 64], [170, 310, 900, 128, 700, 1300, 20, 1129, 600, 64],
+     16, 16, 128, 128, True),
+    ("narrow", [400, 30, 1, 130, 257, 1, 90, 333, 9], [500, 3000, 1200, 130, 2000, 1, 90, 1500, 700], 24, 8, 64, 32, True),
+    ("wide", [100, 33, 1, 200, 65, 31], [1100, 33, 400, 600, 900, 1000], 8, 2, 256, 64, True),
+    ("wide_odd", [100, 33, 1, 200, 65, 31], [1100, 33, 400, 600, 900, 1000], 6, 2, 176, 48, True),
+    ("one_long", [1500], [6000], 8, 2, 128, 64, True),
+    ("tiles_of_one", [40] * 60, [40 + 37 * i % 700 for i in range(60)], 8, 4, 64, 16, True),
+    ("tiles_of_one_128", [40] * 60, [40 + 37 * i % 700 for i in range(60)], 8, 4, 128, 16, True),
+    ("unmasked", [77, 300, 5, 150], [1000, 300, 700, 2222], 8, 4, 96, 32, False),
+    ("decode_32_rows", [7] * 30, [7 + 113 * i % 2000 for i in range(30)], 8, 2, 128, 64, True),
+    ("decode_64_rows", [5, 1, 3, 5, 2] * 6, [5 + 113 * i % 2000 for i in range(30)], 24, 2, 80, 64, True),
+    ("decode_wide_32_rows", [3] * 20, [3 + 113 * i % 2000 for i in range(20)], 8, 1, 256, 48, False),
+    ("group_over_decode", [1, 2, 1, 30, 1], [900, 40, 3000, 600, 1], 160, 2, 64, 32, True),
+    ("long_among_tokens", [1] * 40 + [37], [50 + 97 * i % 3000 for i in range(40)] + [2000], 8, 2, 128, 16, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("case", LARGE, ids=[c[0] for c in LARGE])
+def test_chunk_attention_many_items(case, dtype):
+    from fgw_b200.operators.mha.chunk_attention import paged_chunk_attention
+    _, new, held, _, _, _, page, causal = case
+    held = [max(h, n) for h, n in zip(held, new)]
+    q, k, v, table, lens, cu = attend_case((*case[:2], held, *case[3:]), dtype, seed=21)
+    args = [q.cuda(), k.cuda(), v.cuda()]
+    got = [paged_chunk_attention(*args, *on_gpu(table, lens, cu), page, is_causal=causal) for _ in range(3)]
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    want, spread = torch_attention(*args, table, lens, cu, page, causal)
+    bound = ROUNDOFF[dtype] * (2 * want.abs() + spread) + 2.0 ** -16 * spread + 1e-6
+    if dtype == torch.float16:
+        bound = bound + 2.0 ** -25 * max(held) * float(v.abs().max())
+    err = (got[0].double() - want).abs()
+    assert bool((err <= bound).all()), (float((err / bound).max()), float(err.max()))
+
+
+@pytest.mark.gpu
+def test_chunk_attention_reports_no_device_error_and_zeroes_rows_of_no_request():
+    from fgw_b200 import _native
+    from fgw_b200.operators.mha import chunk_attention
+    q, k, v, table, lens, cu = attend_case(("x", [40, 1, 300], [400, 20, 600], 4, 2, 128, 16, True), torch.bfloat16)
+    q = torch.cat([q[:3], q, q[:5]])  # three rows before the first request, five after the last
+    stream = torch.cuda.current_stream().cuda_stream
+    seen = []
+    launch = _native.chunk_attention
+    try:
+        _native.chunk_attention = lambda p, ws, n, s: (seen.append(ws), launch(p, ws, n, s))
+        out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
+        chunk_attention.paged_chunk_attention(q.cuda(), k.cuda(), v.cuda(), *on_gpu(table, lens, cu + 3), 16, out=out)
+    finally:
+        _native.chunk_attention = launch
+    assert _native.read_error(seen[0], stream) == (_native.OK, 0)
+    assert not out[:3].any() and not out[-5:].any()
+    check_attention(out[3:-5], q[3:-5], k, v, table, lens, cu, 16, True, 128 ** -0.5)
+
+
+@pytest.mark.gpu
+def test_chunk_attention_over_a_pool_past_32_bits():
+    """Cache rows whose element and byte offsets need more than 32 bits."""
+    from fgw_b200.operators.mha.chunk_attention import paged_chunk_attention
+    page, kv_heads, dim = 64, 8, 128
+    pages = (5 << 30) // (page * kv_heads * dim)  # 5 G elements
+    k = torch.zeros((pages * page, kv_heads, dim), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    q, small_k, small_v, table, lens, cu = attend_case(("x", [1, 200], [300, 500], 8, kv_heads, dim, page, True),
+                                                       torch.bfloat16)
+    rows = small_k.shape[0]
+    k[-rows:], v[-rows:] = small_k.cuda(), small_v.cuda()
+    moved = np.where(table >= 0, table + pages - rows // page, -1).astype(np.int32)
+    got = paged_chunk_attention(q.cuda(), k, v, *on_gpu(moved, lens, cu), page)
+    want = paged_chunk_attention(q.cuda(), small_k.cuda(), small_v.cuda(), *on_gpu(table, lens, cu), page)
+    assert torch.equal(got, want)
+
+
 @pytest.mark.gpu
 def test_chunk_attention_peaked_and_scaled():
     """Scores far apart (weights underflow, the running maximum jumps) and another softmax scale."""
