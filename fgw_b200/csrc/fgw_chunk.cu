@@ -8,8 +8,9 @@
 // key head to the decode kernel (fgw_chunk_decode.cu, bound by HBM), the others to the tensor kernel
 // (fgw_chunk_sm100.cu, tcgen05). Lengths are device data, so the host does not know which requests are which: when the
 // requests' average rows fit an item of the decode kernel it launches that alone, which then takes everything (a longer
-// request in several items), else both. The plan (tensor kernel only), decode, tensor and merge kernels follow one
-// another as programmatic dependent launches, so each one's set-up overlaps the one before.
+// request in several items), else both. The plan (for the tensor kernel), tensor, decode and merge kernels follow one
+// another as programmatic dependent launches, so each one's set-up overlaps the one before; the decode kernel needs
+// nothing of the others and starts on the SMs that the tensor kernel leaves first.
 #include <algorithm>
 #include <numeric>
 
@@ -23,7 +24,7 @@ constexpr int kItemCost = 2;           // KV tiles that an item's start and end 
 constexpr int kCutCost = 8;            // KV tiles that cutting items costs (pieces, merge)
 constexpr int kTensorMinUnits = 2;    // units a program's range has at least when every item is cut
 constexpr int kMergeThreads = 256;
-constexpr int kMergeRows[2] = {8, 16};  // rows merged by one CTA, by list
+constexpr int kMergeRows[2] = {4, 32};  // rows merged by one CTA, by list
 
 // Sum over the CTA of each thread's value before it in thread order, and the total.
 template <typename V>
@@ -480,8 +481,8 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_coun
     chunk_plan_kernel<<<1, kPlanListThreads, sizeof(PlanShared), stream>>>(a[1], layout.list);
     err = cudaGetLastError();
   }
-  if (err == cudaSuccess && on[0]) err = launch_chunk_decode(p, a[0], device, stream);
   if (err == cudaSuccess && on[1]) err = launch_chunk_tensor(p, a[1], layout.list, device, stream);
+  if (err == cudaSuccess && on[0]) err = launch_chunk_decode(p, a[0], device, stream);
   if (err != cudaSuccess) return err;
   const unsigned grid = static_cast<unsigned>(a[0].programs * (merge.list[0].parts + merge.list[1].parts));
   return p.dtype == FGW_DTYPE_BFLOAT16

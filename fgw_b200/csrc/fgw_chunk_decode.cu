@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
       a.slots.cuts[blockIdx.x] = {sg.token0, sg.count, sg.hk, range_of(cur, sg.end_u - 1)};
     }
   }
-  grid_dependency_wait();  // so that what follows this kernel follows the plan ahead of it too
+  grid_dependency_wait();  // so that what follows this kernel follows the tensor kernel ahead of it too
 }
 
 template <typename T, int NB, int MT>
@@ -523,7 +523,7 @@ static cudaError_t launch_decode_t(const fgw_chunk_params& p, ChunkArgs a, int d
   CUtensorMap kmap, vmap;
   if (chunk_kv_map(&kmap, p, p.k_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
   if (chunk_kv_map(&vmap, p, p.v_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
-  if (a.split) {  // the plan of the tensor kernel runs ahead; this kernel does not wait for it
+  if (a.split) {  // after the tensor kernel, which it does not wait for until its end
     return launch_after_plan(kernel, static_cast<unsigned>(a.programs), S::kThreads, S::kBytes, stream, kmap, vmap, a);
   }
   kernel<<<a.programs, S::kThreads, S::kBytes, stream>>>(kmap, vmap, a);
