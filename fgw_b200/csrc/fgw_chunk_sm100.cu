@@ -9,8 +9,14 @@
 // overwrites the S columns it came from (TS-form PV). Above 128, O takes 256 columns and an item is one tile.
 // TMEM: S_t at column 128 t, O_A at 256, O_B at 384.
 //
-// Bound by the tensor and special-function units together: a tile pair costs 2048 cycles of MMA at D = 128 and as many of
-// 2^x, and S shares its columns with P, so both must overlap tile against tile.
+// Bound by the softmax chain and its hand-offs: a tile pair costs 2048 cycles of 2^x whatever D is, and 2048 of MMA at
+// D = 128, but a step of the pair takes about 4000 to 4400: the tile's softmax (2400), P seen by the MMA warp and its PV
+// issued (700 to 900), QK issued (400 to 600), S seen (400 to 500), and S shares its columns with P, so these follow one
+// another. Measured: a 4096-token chunk over 32K cached, 32 heads on 8 key heads of 128, 1815 us = 1.14 PFLOP/s. Tried and
+// slower on the same shapes, each time by what the MMA or softmax warps execute per step: two threads per row (four
+// softmax warpgroups; 1902 to 2478 us by the spills), a third score buffer at D = 64 with the MMA warp walking events
+// (D = 64 mix 178 to 192 against 165 us), QK of the next item issued beside the last PV of the one before (no change),
+// a warp that hands out the segments (no change), part of the 2^x on the FMA pipe (184 to 193 against 174 us).
 #include <algorithm>
 
 #include "fgw_chunk.cuh"
