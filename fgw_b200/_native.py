@@ -5,7 +5,7 @@ There is no fallback: if the library is missing or cannot be loaded, every entry
 ``NativeLibraryError`` naming the file, so a GPU box without the built extension fails loudly.
 """
 import ctypes
-import functools
+import importlib.util
 import pathlib
 
 import numpy as np
@@ -211,15 +211,6 @@ class PageParams(ctypes.Structure):
     _fields_ += [("reserved", ctypes.c_int32 * 2)]
 
 
-_FORMATS = {ctypes.c_void_p: "Q", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f",
-            ctypes.c_int32 * 2: "2i"}
-
-
-def struct_format(cls):
-    """``struct`` format of a parameter structure, for callers that pack it as bytes in one call."""
-    return "@" + "".join(_FORMATS[kind] for _, kind in cls._fields_)
-
-
 _LIB = None
 
 
@@ -403,44 +394,28 @@ def paged_cache_gather(params, stream_ptr):
           "fgw_paged_cache_gather")
 
 
-# The params of the calls below are the parameter structure packed as bytes.
-def rotary_append(params, stream_ptr):
-    """``fgw_rotary_append``: rotate the new tokens' queries and keys and append keys and values to the cache."""
-    status = library().fgw_rotary_append(params, stream_ptr)
-    if status:
-        raise FgwError(status, "fgw_rotary_append")
+_BINDING = None
 
 
-def chunk_workspace_size(params):
-    out = ctypes.c_size_t(0)
-    check(library().fgw_chunk_workspace_size(ctypes.byref(params), ctypes.byref(out)), "fgw_chunk_workspace_size")
-    return out.value
-
-
-def chunk_attention(params, workspace_ptr, workspace_bytes, stream_ptr):
-    """``fgw_chunk_attention``: attention of the new tokens over the cache."""
-    status = library().fgw_chunk_attention(params, workspace_ptr, workspace_bytes, stream_ptr)
-    if status:
-        raise FgwError(status, "fgw_chunk_attention")
-
-
-@functools.lru_cache(maxsize=256)
-def page_workspace_bytes(batch, num_pages, copy_count):
-    """``fgw_page_workspace_size`` of a fork or compaction of ``batch`` rows, or (batch 0) of a list of copies."""
-    p = PageParams()
-    p.batch, p.num_pages, p.copy_count = batch, num_pages, copy_count
-    out = ctypes.c_size_t(0)
-    check(library().fgw_page_workspace_size(ctypes.byref(p), ctypes.byref(out)), "fgw_page_workspace_size")
-    return out.value
-
-
-def page_fork(params, workspace_ptr, workspace_bytes, stream_ptr):
-    check(library().fgw_page_fork(params, workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_fork")
-
-
-def page_compact(params, workspace_ptr, workspace_bytes, stream_ptr):
-    check(library().fgw_page_compact(params, workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_compact")
-
-
-def page_copy(params, workspace_ptr, workspace_bytes, stream_ptr):
-    check(library().fgw_page_copy(params, workspace_ptr, workspace_bytes, stream_ptr), "fgw_page_copy")
+def torch_binding():
+    """The compiled binding of the serving-step operators (csrc/fgw_torch.cpp); raises ``NativeLibraryError`` if it
+    cannot be loaded."""
+    global _BINDING
+    if _BINDING is not None:
+        return _BINDING
+    library()  # the same checks, and the file the binding links
+    path = LIB_PATH.parent / "fgw_torch.so"
+    if not path.exists():
+        raise NativeLibraryError(f"{path} is missing: build it with `python -m fgw_b200.build`. There is no CPU fallback "
+                                 "for the serving-step operators.")
+    import torch  # noqa: F401 -- its libraries first
+    spec = importlib.util.spec_from_file_location("fgw_torch", path)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError as exc:
+        raise NativeLibraryError(f"cannot load {path}: {exc}") from exc
+    if module.abi_version() != ABI_VERSION:
+        raise NativeLibraryError(f"{path} was built for another library: rebuild with `python -m fgw_b200.build`")
+    _BINDING = module
+    return module

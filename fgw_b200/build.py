@@ -1,8 +1,9 @@
-"""Build libfgw_mha.so in-tree with nvcc for sm_100a.
+"""Build libfgw_mha.so in-tree with nvcc for sm_100a, and the Python binding of the serving-step operators.
 
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` in parallel; the objects link into
 ``fgw_b200/_lib/libfgw_mha.so`` with the CUDA runtime linked statically, so the library only
-needs the NVIDIA driver at run time. Re-running is incremental (objects newer than their
+needs the NVIDIA driver at run time. ``csrc/fgw_torch.cpp`` becomes ``fgw_b200/_lib/fgw_torch.so`` beside it (a
+Python extension on torch's headers that calls the library). Re-running is incremental (objects newer than their
 sources and headers are kept).
 
     python -m fgw_b200.build [--force] [--jobs N]
@@ -14,6 +15,7 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PACKAGE = pathlib.Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
@@ -22,6 +24,8 @@ INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB_DIR = PACKAGE / "_lib"
 LIB = LIB_DIR / "libfgw_mha.so"
+BINDING = LIB_DIR / "fgw_torch.so"
+BINDING_SOURCE = CSRC / "fgw_torch.cpp"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # Host code keeps separate multiplies and adds (no fused multiply-add contraction): the host split choice
@@ -52,8 +56,27 @@ def _compile(src, obj, extra):
     return proc.stderr
 
 
+def _build_binding():
+    """Compile the Python binding against the torch of this interpreter."""
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], str(INCLUDE)]
+    libraries = cpp_extension.library_paths("cuda")
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = ["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=fgw_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[flag for path in includes for flag in ("-isystem", path)], str(BINDING_SOURCE), "-o", str(tmp),
+           f"-L{LIB_DIR}", *[f"-L{path}" for path in libraries], "-lfgw_mha", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, BINDING)
+
+
 def build(force=False, jobs=None, verbose_ptxas=False):
-    """Compile every kernel translation unit and link the shared library; returns its path."""
+    """Compile every kernel translation unit, link the shared library and build the binding; returns the library's path."""
     BUILD.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
@@ -75,6 +98,8 @@ def build(force=False, jobs=None, verbose_ptxas=False):
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
         os.replace(tmp, LIB)
+    if force or _stale(BINDING, BINDING_SOURCE, sorted(INCLUDE.glob("*.h"))):
+        _build_binding()
     if verbose_ptxas:
         for name, text in sorted(logs.items()):
             print(f"== {name}\n{text}")

@@ -5,17 +5,12 @@ keys and writes keys and values where ``paged_chunk_attention`` reads them, in o
 callers bring a filled cache.
 """
 import math
-import struct
 
 import torch
 
 from fgw_b200 import _native
-from fgw_b200.operators.mha.chunk_attention import (_DTYPES, aligned, check_ragged, on_device, output_like,
-                                                    token_stride)
-from fgw_b200.operators.mha.kernels.mha_paged_fwd_sm100 import _current_stream
 
 SCALINGS = (None, "linear", "ntk", "yarn")
-_PACK = struct.Struct(_native.struct_format(_native.RotaryParams)).pack
 
 
 def rotary_table(positions, rotary_dim, base=10000.0, scaling=None, factor=1.0, original_positions=None,
@@ -72,31 +67,8 @@ def rotary_append(q, k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seql
     ``paged_chunk_attention``, which takes the result. The i-th of request b's n new tokens has position
     ``cache_seqlens[b] - n + i``. Pairs are values (i, i + rotary_dim / 2) of a head, or (2 i, 2 i + 1) when
     ``interleaved``; values from rotary_dim on pass. ``out`` may be ``q``. Rows of no request, and positions outside
-    the page table or ``cos_sin``, give zeros and append nothing.
+    the page table or ``cos_sin``, give zeros and append nothing. Raises
+    ValueError for tensors that do not fit this, before any launch.
     """
-    tokens, heads, dim, kv_heads, rows, batch, width = check_ragged(q, k_cache, v_cache, block_table, cache_seqlens,
-                                                                    cu_seqlens_q, page_size)
-    if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape:
-        raise ValueError("Expected k and v [T,Hkv,D]")
-    if k.dtype != q.dtype or v.dtype != q.dtype or cos_sin.dtype != torch.float32:
-        raise ValueError("k and v take q's type, cos_sin float32")
-    if cos_sin.dim() != 2:
-        raise ValueError("cos_sin must be [positions, rotary_dim]")
-    positions, rotary_dim = cos_sin.shape
-    if positions <= 0 or rotary_dim < 2 or rotary_dim > dim or rotary_dim % 2:
-        raise ValueError("cos_sin must have a row and rotary_dim be even and at most D")
-    device = q.get_device()
-    if k.get_device() != device or v.get_device() != device or cos_sin.get_device() != device:
-        raise ValueError("every tensor must be on the same CUDA device")
-    if not cos_sin.is_contiguous():
-        raise ValueError("kernel inputs must be contiguous")
-    out, out_stride = output_like(q, out)
-    q_stride, k_stride, v_stride = token_stride(q, "q"), token_stride(k, "k"), token_stride(v, "v")
-    if not tokens:
-        return out
-    params = _PACK(*aligned(q, k, v, out, k_cache, v_cache), block_table.data_ptr(), cache_seqlens.data_ptr(),
-                   cu_seqlens_q.data_ptr(), cos_sin.data_ptr(), tokens, rows, q_stride, k_stride, v_stride, out_stride,
-                   batch, heads, kv_heads, dim, rotary_dim, min(positions, (1 << 31) - 1), width, page_size,
-                   _DTYPES[q.dtype], 1 if interleaved else 0, 0, 0)
-    on_device(device, _native.rotary_append, params, _current_stream(device))
-    return out
+    return _native.torch_binding().rotary_append(q, k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens_q,
+                                                 cos_sin, page_size, interleaved, out)

@@ -175,20 +175,26 @@ def test_chunk_attention_many_items(case, dtype):
 
 @pytest.mark.gpu
 def test_chunk_attention_reports_no_device_error_and_zeroes_rows_of_no_request():
+    import ctypes
+
     from fgw_b200 import _native
-    from fgw_b200.operators.mha import chunk_attention
     q, k, v, table, lens, cu = attend_case(("x", [40, 1, 300], [400, 20, 600], 4, 2, 128, 16, True), torch.bfloat16)
     q = torch.cat([q[:3], q, q[:5]])  # three rows before the first request, five after the last
-    stream = torch.cuda.current_stream().cuda_stream
-    seen = []
-    launch = _native.chunk_attention
-    try:
-        _native.chunk_attention = lambda p, ws, n, s: (seen.append(ws), launch(p, ws, n, s))
-        out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
-        chunk_attention.paged_chunk_attention(q.cuda(), k.cuda(), v.cuda(), *on_gpu(table, lens, cu + 3), 16, out=out)
-    finally:
-        _native.chunk_attention = launch
-    assert _native.read_error(seen[0], stream) == (_native.OK, 0)
+    args = [q.cuda(), k.cuda(), v.cuda(), *on_gpu(table, lens, cu + 3)]
+    out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
+    p = _native.ChunkParams()  # by the C ABI, whose caller has the workspace to read the status from
+    for name, t in zip(("q", "k_cache", "v_cache", "block_table", "cache_seqlens", "cu_seqlens_q", "out"), (*args, out)):
+        setattr(p, name, t.data_ptr())
+    for name, value in dict(tokens=q.shape[0], pool_rows=k.shape[0], q_stride=512, out_stride=512, batch=3, heads=4,
+                            kv_heads=2, head_dim=128, table_width=table.shape[1], page_size=16,
+                            dtype=_native.DTYPE_BFLOAT16, causal=1, softmax_scale=128 ** -0.5).items():
+        setattr(p, name, value)
+    size = ctypes.c_size_t()
+    lib, stream = _native.library(), torch.cuda.current_stream().cuda_stream
+    assert lib.fgw_chunk_workspace_size(ctypes.byref(p), ctypes.byref(size)) == 0
+    workspace = torch.full((size.value,), 255, dtype=torch.uint8, device="cuda")  # whatever it holds
+    assert lib.fgw_chunk_attention(ctypes.byref(p), workspace.data_ptr(), size.value, stream) == 0
+    assert _native.read_error(workspace.data_ptr(), stream) == (_native.OK, 0)
     assert not out[:3].any() and not out[-5:].any()
     check_attention(out[3:-5], q[3:-5], k, v, table, lens, cu, 16, True, 128 ** -0.5)
 
