@@ -128,8 +128,11 @@ __global__ void __launch_bounds__(kPlanListThreads)
   const bool mine = tid < programs;
   auto units_of = [&](int round) {  // of this program's item in a round, 0 when it has none
     const int item = round * programs + ((round & 1) ? programs - 1 - tid : tid);
-    return mine && item < items ? sorted[item / a.kv_heads].z : 0;
+    return mine && item < items ? sorted[a.by_kv_heads.quotient(item)].z : 0;
   };
+  const long long quotient = divide(total, programs);
+  const int remainder = static_cast<int>(total - quotient * programs);
+  const long long fair = mine ? quotient + (tid < remainder ? 1 : 0) : 0;  // units of an equal share
   const int all_rounds = (items + programs - 1) / programs;
   int rounds = 0, ranges = programs;
   long long load = 0;
@@ -138,15 +141,14 @@ __global__ void __launch_bounds__(kPlanListThreads)
       const int units = units_of(r);
       load += units > 0 ? units + kItemCost : 0;
     }
-    const long long equal = (total + static_cast<long long>(items) * kItemCost) / programs;
+    const long long equal = divide(total + static_cast<long long>(items) * kItemCost, programs);
     if (__syncthreads_and(load <= equal + equal / 20 + kCutCost)) {
       rounds = all_rounds;
     } else {
-      const long long share = mine ? program_start(total, programs, tid + 1) - program_start(total, programs, tid) : 0;
       load = 0;
       while (static_cast<long long>(rounds + 1) * programs <= items) {
         const int units = units_of(rounds);
-        if (!__syncthreads_and(!mine || load + units <= share)) break;
+        if (!__syncthreads_and(load + units <= fair)) break;
         load += units;
         ++rounds;
       }
@@ -158,9 +160,10 @@ __global__ void __launch_bounds__(kPlanListThreads)
   const bool none = cut == items;
   long long share = 0;
   if (!none && rounds > 0) {
-    share = program_start(total, programs, tid + 1) - program_start(total, programs, tid) - load;
+    share = fair - load;
   } else if (!none && tid < ranges) {
-    share = program_start(total, ranges, tid + 1) - program_start(total, ranges, tid);
+    const long long each = divide(total, ranges);
+    share = each + (tid < total - each * ranges ? 1 : 0);
   }
   long long rest;
   const long long before = block_scan(mine ? share : 0ll, rest, sh.scan_l);
@@ -168,8 +171,8 @@ __global__ void __launch_bounds__(kPlanListThreads)
     long long u = total;
     int item = 0, off = 0;
     if (!none) {
-      const int cut_row = cut / a.kv_heads;
-      u = prefix[cut_row] + static_cast<long long>(cut % a.kv_heads) * sorted[cut_row].z + before;
+      const int cut_row = a.by_kv_heads.quotient(cut);
+      u = prefix[cut_row] + static_cast<long long>(cut - cut_row * a.kv_heads) * sorted[cut_row].z + before;
       int lo = 0, hi = rows - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -182,8 +185,9 @@ __global__ void __launch_bounds__(kPlanListThreads)
       if (u < total) {
         const int units = sorted[lo].z;
         const long long within = u - prefix[lo];
-        item = lo * a.kv_heads + static_cast<int>(within / units);
-        off = static_cast<int>(within % units);
+        const int hk = static_cast<int>(divide(within, units));
+        item = lo * a.kv_heads + hk;
+        off = static_cast<int>(within - static_cast<long long>(hk) * units);
       }
     }
     list.prog_u[tid] = u;
@@ -454,6 +458,7 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_coun
   a[0].programs = std::min(sm_count, kStreamMaxPrograms);
   a[0].by_page = FastDiv(p.page_size);
   a[0].by_group = FastDiv(a[0].group);
+  a[0].by_kv_heads = FastDiv(p.kv_heads);
   a[0].small_rows = decode_rows(p);
   a[0].split = on[0] && on[1] ? 1 : 0;
   a[0].scale_log2 = p.softmax_scale * kLog2e;

@@ -57,7 +57,7 @@ struct ChunkArgs {
   long long tokens, q_stride, out_stride;
   int batch, heads, kv_heads, group, dim, width, page, causal, box_rows, programs;
   int tokens_per_item;
-  FastDiv by_page, by_group, by_item_tokens;
+  FastDiv by_page, by_group, by_item_tokens, by_kv_heads;
   int small_rows;  // rows of a decode item; requests of at most so many go to the decode kernel
   int split;       // requests go by their rows; otherwise everything is the launched kernel's
   float scale_log2;

@@ -90,16 +90,6 @@ struct DecodeCursor {
   int remainder;
 };
 
-// x / y for x >= 0 and y > 0; nearly always the cheap 32-bit one.
-__device__ __forceinline__ long long divide(long long x, int y) {
-  if (x <= 0x7fffffffll) return static_cast<long long>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
-  return x / y;
-}
-// First unit of program p (program_start with the quotient already taken).
-__device__ __forceinline__ long long range_start(long long quotient, int remainder, int p) {
-  return quotient * p + min(p, remainder);
-}
-
 // The program that holds unit u.
 __device__ __forceinline__ int range_of(const DecodeCursor& k, long long u) {
   const long long longer = k.remainder * (k.quotient + 1);

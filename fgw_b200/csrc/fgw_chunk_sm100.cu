@@ -74,10 +74,11 @@ __device__ __forceinline__ bool next_segment(const ChunkArgs& a, const ChunkList
     if (k.u >= k.u_end) return false;
     item = k.item;
   }
-  const int4 row = list.rows[item / a.kv_heads];
+  const int list_row = a.by_kv_heads.quotient(item);
+  const int4 row = list.rows[list_row];
   const int units = row.z, first = whole ? 0 : k.off;
   const int count = whole ? units : static_cast<int>(min(static_cast<long long>(units - first), k.u_end - k.u));
-  make_segment<128>(a, s, row.x, item % a.kv_heads, new_tokens(a.cu, a.tokens, row.x),
+  make_segment<128>(a, s, row.x, item - list_row * a.kv_heads, new_tokens(a.cu, a.tokens, row.x),
                     held_tokens(a.lens, row.x, a.width, a.page), row.y, units, first, count);
   if (!whole) {
     s.end_u = k.u - first + units;

@@ -28,6 +28,16 @@ struct FastDiv {
   }
 };
 
+// x / y for x >= 0 and y > 0; nearly always the cheap 32-bit one.
+__device__ __forceinline__ long long divide(long long x, int y) {
+  if (x <= 0x7fffffffll) return static_cast<long long>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
+  return x / y;
+}
+// First unit of program p (program_start with the quotient already taken).
+__device__ __forceinline__ long long range_start(long long quotient, int remainder, int p) {
+  return quotient * p + min(p, remainder);
+}
+
 // The last request whose offset is at most t, by a converged warp; 0 where there is none.
 __device__ __forceinline__ int find_request(const int32_t* cu, int batch, long long t, int lane) {
   int lo = 0, hi = batch;  // the answer is in [lo, hi)
