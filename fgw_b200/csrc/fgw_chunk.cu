@@ -24,7 +24,7 @@ constexpr int kItemCost = 2;           // KV tiles that an item's start and end 
 constexpr int kCutCost = 8;            // KV tiles that cutting items costs (pieces, merge)
 constexpr int kTensorMinUnits = 2;    // units a program's range has at least when every item is cut
 constexpr int kMergeThreads = 256;
-constexpr int kMergeRows[2] = {4, 32};  // rows merged by one CTA, by list
+constexpr int kMergeRows[2] = {4, 64};  // rows merged by one CTA, by list
 
 // Sum over the CTA of each thread's value before it in thread order, and the total.
 template <typename V>
