@@ -18,10 +18,13 @@
 
 namespace fgw {
 
-constexpr int kPlanListThreads = 1024;
+constexpr int kPlanListThreads = 512;  // against 1024: 9.0 -> 8.3 us of plan for a mixed step, 256 no better
 constexpr int kPlanSorted = 2048;     // rows of a list sorted in shared memory; longer lists keep the request order
-constexpr int kItemCost = 2;           // KV tiles that an item's start and end cost, in the choice of whole rounds
-constexpr int kCutCost = 8;            // KV tiles that cutting items costs (pieces, merge)
+// What the tensor kernel's time is dealt by, in quarters of a KV tile's step of two query tiles. From a fit to the times of
+// its CTAs (D = 64: 1.93 us per step of two query tiles, 1.52 us of one, 4.5 us per item; D = 128: 2.95, 2.0 and 4.1 us).
+constexpr int kStepCost = 4, kOneTileStepCost = 3;
+constexpr int kItemCost = 9;           // an item's start and end
+constexpr int kCutCost = 32;           // cutting items: pieces, merge
 constexpr int kTensorMinUnits = 2;    // units a program's range has at least when every item is cut
 constexpr int kMergeThreads = 256;
 constexpr int kMergeRows[2] = {4, 64};  // rows merged by one CTA, by list
@@ -53,15 +56,19 @@ __device__ __forceinline__ V block_scan(V v, V& total, V* shared) {
   return sum - v + (warp > 0 ? shared[warp - 1] : V(0));
 }
 
-// The tensor kernel's work list: the items by descending units; whole rounds of one item per program in snake order,
-// either all of them, where that comes within 5 % and what cutting costs of an equal share, or as many as stay within each
-// program's share, the rest cut into a contiguous range of units per program that fills its share up.
+// The tensor kernel's work list: the items by descending cost, dealt in whole rounds of one item per program: in snake
+// order, the last round to the programs with the least load first. Where the longest program would exceed an equal share
+// by more than 5 % and what cutting costs, only as many rounds are whole as stay within each program's share, and the rest
+// is cut into a contiguous range of units per program that fills its share up. The last round by load, against snake
+// order throughout: a batch of prompts 64.6 -> 58.3 us (CTAs of 28 to 53 us -> 28 to 45), single tokens and chunks
+// mixed 160.9 -> 158.4 us.
 struct PlanShared {
   long long scan_l[32];
   int scan_i[32];
-  int4 raw[kPlanSorted], rows[kPlanSorted];
+  int4 raw[kPlanSorted], rows[kPlanSorted];  // {request, first token, units, cost}
   long long prefix[kPlanSorted + 1];
   int first[kPlanSorted + 1];
+  alignas(16) uint32_t loads[kStreamMaxPrograms];
 };
 
 __global__ void __launch_bounds__(kPlanListThreads)
@@ -93,11 +100,13 @@ __global__ void __launch_bounds__(kPlanListThreads)
     const int len = held_tokens(a.lens, b, a.width, a.page);
     for (int r = begin + lane; r < end; r += 32) {
       const int t0 = (r - begin) * a.tokens_per_item;
-      raw[r] = make_int4(b, t0, item_units<128>(a, count, len, t0), 0);
+      const int units = item_units<128>(a, count, len, t0);
+      const bool one_tile = a.dim <= 128 && 2 * (count - t0) <= a.tokens_per_item;
+      raw[r] = make_int4(b, t0, units, units * (one_tile ? kOneTileStepCost : kStepCost) + kItemCost);
     }
   }
   __syncthreads();
-  // by descending units (ties: in order), so that whole items are dealt longest first; with fewer items than programs
+  // by descending cost (ties: in order), so that whole items are dealt longest first; with fewer items than programs
   // all are cut and the order does not matter
   const int programs = a.programs;
   const int items = rows * a.kv_heads;
@@ -108,7 +117,7 @@ __global__ void __launch_bounds__(kPlanListThreads)
     int rank = r;
     if (order) {
       rank = 0;
-      for (int s = 0; s < rows; ++s) rank += (raw[s].z > row.z || (raw[s].z == row.z && s < r)) ? 1 : 0;
+      for (int s = 0; s < rows; ++s) rank += (raw[s].w > row.w || (raw[s].w == row.w && s < r)) ? 1 : 0;
     }
     sorted[rank] = row;
     if (small) list.rows[rank] = row;
@@ -126,32 +135,47 @@ __global__ void __launch_bounds__(kPlanListThreads)
   if (tid == 0) prefix[rows] = total;
   __syncthreads();
   const bool mine = tid < programs;
-  auto units_of = [&](int round) {  // of this program's item in a round, 0 when it has none
+  auto item_of = [&](int round) {  // this program's item in a round in snake order, {0, 0, 0, 0} when it has none
     const int item = round * programs + ((round & 1) ? programs - 1 - tid : tid);
-    return mine && item < items ? sorted[a.by_kv_heads.quotient(item)].z : 0;
+    return mine && item < items ? sorted[a.by_kv_heads.quotient(item)] : make_int4(0, 0, 0, 0);
   };
   const long long quotient = divide(total, programs);
   const int remainder = static_cast<int>(total - quotient * programs);
   const long long fair = mine ? quotient + (tid < remainder ? 1 : 0) : 0;  // units of an equal share
   const int all_rounds = (items + programs - 1) / programs;
-  int rounds = 0, ranges = programs;
+  int rounds = 0, snake = 0, ranges = programs, last = items;
   long long load = 0;
   if (items > programs) {
-    for (int r = 0; r < all_rounds; ++r) {
-      const int units = units_of(r);
-      load += units > 0 ? units + kItemCost : 0;
+    for (int r = 0; r + 1 < all_rounds; ++r) load += item_of(r).w;
+    const uint32_t have = static_cast<uint32_t>(min(load, 0xfffffffell));
+    if (tid < kStreamMaxPrograms) sh.loads[tid] = mine ? have : 0xffffffffu;
+    __syncthreads();
+    if (mine) {
+      int rank = 0;
+#pragma unroll 4
+      for (int p = 0; p < programs; p += 4) {
+        const uint4 four = *reinterpret_cast<const uint4*>(&sh.loads[p]);
+        rank += (four.x < have || (four.x == have && p < tid)) + (four.y < have || (four.y == have && p + 1 < tid)) +
+                (four.z < have || (four.z == have && p + 2 < tid)) + (four.w < have || (four.w == have && p + 3 < tid));
+      }
+      last = min((all_rounds - 1) * programs + rank, items);
+      if (last < items) load += sorted[a.by_kv_heads.quotient(last)].w;
     }
-    const long long equal = divide(total + static_cast<long long>(items) * kItemCost, programs);
-    if (__syncthreads_and(load <= equal + equal / 20 + kCutCost)) {
+    long long all_cost;
+    block_scan(mine ? load : 0ll, all_cost, sh.scan_l);
+    const long long equal = divide(all_cost, programs);
+    if (__syncthreads_and(!mine || load <= equal + equal / 20 + kCutCost)) {
       rounds = all_rounds;
+      snake = all_rounds - 1;
     } else {
       load = 0;
       while (static_cast<long long>(rounds + 1) * programs <= items) {
-        const int units = units_of(rounds);
+        const int units = item_of(rounds).z;
         if (!__syncthreads_and(load + units <= fair)) break;
         load += units;
         ++rounds;
       }
+      snake = rounds;
     }
   } else {
     ranges = static_cast<int>(max(1ll, min(static_cast<long long>(programs), total / kTensorMinUnits)));
@@ -169,7 +193,7 @@ __global__ void __launch_bounds__(kPlanListThreads)
   const long long before = block_scan(mine ? share : 0ll, rest, sh.scan_l);
   if (mine) {
     long long u = total;
-    int item = 0, off = 0;
+    int item = last, off = 0;  // the last round's item, else the first of the cut range
     if (!none) {
       const int cut_row = a.by_kv_heads.quotient(cut);
       u = prefix[cut_row] + static_cast<long long>(cut - cut_row * a.kv_heads) * sorted[cut_row].z + before;
@@ -198,6 +222,7 @@ __global__ void __launch_bounds__(kPlanListThreads)
     list.prog_u[programs] = total;
     list.meta->items = items;
     list.meta->rounds = rounds;
+    list.meta->snake = snake;
   }
 }
 

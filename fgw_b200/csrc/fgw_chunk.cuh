@@ -33,16 +33,17 @@ struct ChunkSlots {
 // The tensor kernel's work list, written by the plan kernel.
 struct ChunkMeta {
   int items;      // rows of the list x key heads
-  int rounds;     // whole rounds dealt in snake order
-  int pad[2];
+  int rounds;     // rounds of whole items: snake order, then, when all items are whole, a round dealt by load
+  int snake;      // rounds of them in snake order
+  int pad;
 };
 struct ChunkList {
   ChunkMeta* meta;
-  int4* rows;              // sorted: {request, first token in the request, units, 0}
+  int4* rows;              // sorted: {request, first token in the request, units, cost}
   int4* unsorted;          // plan scratch, as are prefix and first
   long long* prefix;       // [rows + 1] first unit of each row's first item
   int32_t* first;          // [batch + 1] first row of each request
-  int32_t* prog_item;      // [programs] first item of the program's cut range
+  int32_t* prog_item;      // [programs] the round dealt by load, or the first item of the program's cut range
   int32_t* prog_off;       // [programs] units of that item before the range
   long long* prog_u;       // [programs + 1] first unit of the range
   int max_rows;
