@@ -533,8 +533,7 @@ static cudaError_t launch_decode_nb(const fgw_chunk_params& p, const ChunkArgs& 
     case 32:
       return launch_decode_t<T, NB, 2>(p, a, device, stream);
     default:
-      if constexpr (NB <= 2) return launch_decode_t<T, NB, 4>(p, a, device, stream);
-      return cudaErrorInvalidValue;
+      return launch_decode_t<T, NB, 4>(p, a, device, stream);
   }
 }
 
