@@ -149,6 +149,11 @@ LARGE = [
     ("decode_32_rows", [7] * 30, [7 + 113 * i % 2000 for i in range(30)], 8, 2, 128, 64, True),
     ("decode_64_rows", [5, 1, 3, 5, 2] * 6, [5 + 113 * i % 2000 for i in range(30)], 24, 2, 80, 64, True),
     ("decode_wide_32_rows", [3] * 20, [3 + 113 * i % 2000 for i in range(20)], 8, 1, 256, 48, False),
+    ("decode_wide_64_rows", [8, 5, 1, 7] * 6, [8 + 113 * i % 2000 for i in range(24)], 8, 1, 256, 48, False),
+    ("decode_wide_odd_64_rows", [5, 8, 2] * 7, [8 + 113 * i % 1500 for i in range(21)], 16, 2, 176, 16, True),
+    ("rounds_by_load", [90 + 53 * i % 400 for i in range(40)], [500 + 211 * i % 1700 for i in range(40)], 8, 8, 128, 64, True),
+    ("rounds_by_load_narrow", [30 + 53 * i % 300 for i in range(40)], [400 + 211 * i % 1700 for i in range(40)], 6, 6, 48, 32,
+     True),
     ("group_over_decode", [1, 2, 1, 30, 1], [900, 40, 3000, 600, 1], 160, 2, 64, 32, True),
     ("long_among_tokens", [1] * 40 + [37], [50 + 97 * i % 3000 for i in range(40)] + [2000], 8, 2, 128, 16, True),
 ]
