@@ -64,6 +64,7 @@ EXPORTED = (
     "fgw_rotary_append",
     "fgw_chunk_workspace_size",
     "fgw_chunk_attention",
+    "fgw_chunk_selftest_wait",
     "fgw_page_workspace_size",
     "fgw_page_fork",
     "fgw_page_compact",
@@ -271,6 +272,8 @@ def library():
         fn = getattr(lib, name)
         fn.argtypes = [vp, ctypes.POINTER(ctypes.c_size_t)]
         fn.restype = ctypes.c_int
+    lib.fgw_chunk_selftest_wait.argtypes = [vp, ctypes.c_int, vp, ctypes.c_size_t, vp]
+    lib.fgw_chunk_selftest_wait.restype = ctypes.c_int
     for name in ("fgw_chunk_attention", "fgw_page_fork", "fgw_page_compact", "fgw_page_copy"):
         fn = getattr(lib, name)
         fn.argtypes = [vp, vp, ctypes.c_size_t, vp]

@@ -488,7 +488,8 @@ int fgw_chunk_workspace_size(const fgw_chunk_params* params, size_t* bytes) {
   return st;
 }
 
-int fgw_chunk_attention(const fgw_chunk_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+static int chunk_attention(const fgw_chunk_params* params, int short_boxes, void* workspace, size_t workspace_bytes,
+                           void* stream) {
   if (params == nullptr) return FGW_ERR_INVALID_ARGUMENT;
   int st = chunk_validate(*params);
   if (st != FGW_OK || params->tokens == 0) return st;
@@ -499,8 +500,18 @@ int fgw_chunk_attention(const fgw_chunk_params* params, void* workspace, size_t 
   int device = 0, sms = 0;
   st = current_device(&device, &sms);
   if (st != FGW_OK) return st;
-  const cudaError_t err = launch_chunk(*params, workspace, sms, device, static_cast<cudaStream_t>(stream));
+  const cudaError_t err = launch_chunk(*params, short_boxes, workspace, sms, device, static_cast<cudaStream_t>(stream));
   return err == cudaSuccess ? FGW_OK : FGW_ERR_CUDA;
+}
+
+int fgw_chunk_attention(const fgw_chunk_params* params, void* workspace, size_t workspace_bytes, void* stream) {
+  return chunk_attention(params, 0, workspace, workspace_bytes, stream);
+}
+
+int fgw_chunk_selftest_wait(const fgw_chunk_params* params, int short_loads, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  if (short_loads < 0 || short_loads > 3) return FGW_ERR_INVALID_ARGUMENT;
+  return chunk_attention(params, short_loads, workspace, workspace_bytes, stream);
 }
 
 static int page_workspace_size(const fgw_page_params* params, int op, size_t* bytes) {

@@ -383,7 +383,7 @@ int chunk_validate_pointers(const fgw_chunk_params& p) {
 
 int chunk_box_rows(int page, int keys) { return std::gcd(page, keys); }
 
-CUresult chunk_kv_map(CUtensorMap* map, const fgw_chunk_params& p, const void* base, int box_rows) {
+static CUresult chunk_kv_map(CUtensorMap* map, const fgw_chunk_params& p, const void* base, int box_rows) {
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.head_dim), static_cast<cuuint64_t>(p.kv_heads),
                               static_cast<cuuint64_t>(p.pool_rows)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.head_dim) * 2,
@@ -395,6 +395,11 @@ CUresult chunk_kv_map(CUtensorMap* map, const fgw_chunk_params& p, const void* b
   return encode_tiled_cached(map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+CUresult chunk_kv_maps(CUtensorMap* kmap, CUtensorMap* vmap, const fgw_chunk_params& p, const ChunkArgs& a) {
+  const CUresult err = chunk_kv_map(kmap, p, p.k_cache, a.box_rows / (a.short_boxes & 1 ? 2 : 1));
+  return err != CUDA_SUCCESS ? err : chunk_kv_map(vmap, p, p.v_cache, a.box_rows / (a.short_boxes & 2 ? 2 : 1));
 }
 
 // Rows of a decode item (16, 32 or 64): enough for the requests' average rows where that is at all possible, else (chunks
@@ -463,7 +468,8 @@ static ChunkLayout chunk_layout(const fgw_chunk_params& p, uint8_t* const begin)
 
 size_t chunk_workspace_bytes(const fgw_chunk_params& p) { return chunk_layout(p, nullptr).bytes; }
 
-cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_count, int device, cudaStream_t stream) {
+cudaError_t launch_chunk(const fgw_chunk_params& p, int short_boxes, void* workspace, int sm_count, int device,
+                         cudaStream_t stream) {
   const ChunkLayout layout = chunk_layout(p, static_cast<uint8_t*>(workspace));
   const bool on[2] = {decode_on(p), tensor_on(p)};
   ChunkArgs a[2] = {};
@@ -490,6 +496,7 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_coun
   a[0].small_rows = decode_rows(p);
   a[0].split = on[0] && on[1] ? 1 : 0;
   a[0].scale_log2 = p.softmax_scale * kLog2e;
+  a[0].short_boxes = short_boxes;
   a[0].budget_ns = static_cast<uint64_t>(p.wait_budget_ms > 0 ? p.wait_budget_ms : 2000) * 1000000ull;
   a[1] = a[0];
   MergeArgs merge = {};

@@ -16,6 +16,9 @@
 namespace fgw {
 
 constexpr int kTensorTileRows = 128;
+// The limit of the waits with which a CTA leaves no copy in flight. They follow loads that are already issued, so they
+// end at once unless a load is lost.
+constexpr uint64_t kDrainBudgetNs = 100000000ull;
 
 // The item whose first piece a program holds when that item goes on in later programs; last < 0: none.
 struct ChunkCut {
@@ -61,6 +64,7 @@ struct ChunkArgs {
   FastDiv by_page, by_group, by_item_tokens, by_kv_heads;
   int small_rows;  // rows of a decode item; requests of at most so many go to the decode kernel
   int split;       // requests go by their rows; otherwise everything is the launched kernel's
+  int short_boxes; // self-test, host only: K's (1) and V's (2) boxes have half the rows that the kernels wait for
   float scale_log2;
   uint64_t budget_ns;
   ChunkSlots slots;
@@ -139,8 +143,8 @@ cudaError_t launch_chunk_decode(const fgw_chunk_params& p, ChunkArgs a, int devi
 cudaError_t launch_chunk_tensor(const fgw_chunk_params& p, ChunkArgs a, const ChunkList& list, int device,
                                 cudaStream_t stream);
 
-// K/V tensor map {D, kv heads, pool rows} with boxes of 64 values x box_rows tokens, 128-byte swizzle.
-CUresult chunk_kv_map(CUtensorMap* map, const fgw_chunk_params& p, const void* base, int box_rows);
+// K and V tensor maps {D, kv heads, pool rows} with boxes of 64 values x a.box_rows tokens, 128-byte swizzle.
+CUresult chunk_kv_maps(CUtensorMap* kmap, CUtensorMap* vmap, const fgw_chunk_params& p, const ChunkArgs& a);
 // Rows per box: boxes never cross a page or a tile of `keys` tokens.
 int chunk_box_rows(int page, int keys);
 

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
     const uint32_t box_bytes = a.box_rows * 128;
     const uint64_t policy = l2_policy_evict_first();
     bool ok = true;
-    uint32_t st = 0, phase = 0;
+    uint32_t st = 0, phase = 0, issued = 0;  // issued: stages given to loads
     while (ok && next_segment<BN>(a, cur, sg)) {
       const int32_t* table = a.table + static_cast<long long>(sg.b) * a.width;
       for (int j = 0; j < sg.n && ok; ++j) {
@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
           break;
         }
         if (lane == 0) mbar_arrive_expect_tx(&full[st], loads * box_bytes);
+        ++issued;
         __syncwarp();
         if (load) {
           uint8_t* dst = smem + (2 * st + which) * S::kTileBytes + blk * S::kBlockBytes + box * box_bytes;
@@ -273,6 +274,10 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
         }
       }
     }
+    // Leave no copy in flight, whichever role gave up: the last load of every stage lands before the CTA may end.
+    for (uint32_t i = issued > NS ? issued - NS : 0; i < issued; ++i) {
+      mbar_wait(&full[i % NS], (i / NS) & 1, kDrainBudgetNs);
+    }
     return;
   }
 
@@ -282,6 +287,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
   const uint32_t base = smem_u32(smem);
   const uint32_t q_at = base + S::kQ, p_at = base + S::kP;
   uint32_t st = 0, phase = 0;
+  bool aborted = false;  // uniform over the consumers
   while (next_segment<BN>(a, cur, sg)) {
     int seen[MT][2];
     long long out_at[MT][2];  // element offset of the row's output, -1: no row
@@ -385,7 +391,10 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
         }
       }
       named_barrier_sync(1, kConsumers);
-      if (*abort_flag != 0) return;  // all warps read it here, between the same two barriers
+      if (*abort_flag != 0) {  // all warps read it here, between the same two barriers
+        aborted = true;
+        break;
+      }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -457,6 +466,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
         phase ^= 1;
       }
     }
+    if (aborted) break;
     // the rows' sums over all warps (row_max's readers have passed the last barrier)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -505,7 +515,8 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
       a.slots.cuts[blockIdx.x] = {sg.token0, sg.count, sg.hk, range_of(cur, sg.end_u - 1)};
     }
   }
-  grid_dependency_wait();  // so that what follows this kernel follows the tensor kernel ahead of it too
+  // So that what follows this kernel follows the tensor kernel ahead of it too; CTAs that gave up come here as well.
+  grid_dependency_wait();
 }
 
 template <typename T, int NB, int MT>
@@ -516,8 +527,7 @@ static cudaError_t launch_decode_t(const fgw_chunk_params& p, ChunkArgs a, int d
   if (err != cudaSuccess) return err;
   a.box_rows = chunk_box_rows(p.page_size, S::kBN);
   CUtensorMap kmap, vmap;
-  if (chunk_kv_map(&kmap, p, p.k_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
-  if (chunk_kv_map(&vmap, p, p.v_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
+  if (chunk_kv_maps(&kmap, &vmap, p, a) != CUDA_SUCCESS) return cudaErrorInvalidValue;
   if (a.split) {  // after the tensor kernel, which it does not wait for until its end
     return launch_after_plan(kernel, static_cast<unsigned>(a.programs), S::kThreads, S::kBytes, stream, kmap, vmap, a);
   }

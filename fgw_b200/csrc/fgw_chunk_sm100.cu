@@ -708,8 +708,7 @@ static cudaError_t launch_tensor_t(const fgw_chunk_params& p, ChunkArgs a, const
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
     return cudaErrorInvalidValue;
   }
-  if (chunk_kv_map(&kmap, p, p.k_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
-  if (chunk_kv_map(&vmap, p, p.v_cache, a.box_rows) != CUDA_SUCCESS) return cudaErrorInvalidValue;
+  if (chunk_kv_maps(&kmap, &vmap, p, a) != CUDA_SUCCESS) return cudaErrorInvalidValue;
   return launch_after_plan(kernel, static_cast<unsigned>(a.programs), S::kThreads, S::kBytes, stream, qmap, kmap, vmap,
                            a, list);
 }

@@ -108,7 +108,8 @@ constexpr int kMaxGroup = 128;  // query heads that may share a key head
 int chunk_validate(const fgw_chunk_params& p);
 int chunk_validate_pointers(const fgw_chunk_params& p);
 size_t chunk_workspace_bytes(const fgw_chunk_params& p);
-cudaError_t launch_chunk(const fgw_chunk_params& p, void* workspace, int sm_count, int device, cudaStream_t stream);
+cudaError_t launch_chunk(const fgw_chunk_params& p, int short_boxes, void* workspace, int sm_count, int device,
+                         cudaStream_t stream);
 // Page-table operators (fgw_pages.cu).
 enum PageOp { kPageFork = 0, kPageCompact = 1, kPageCopy = 2 };
 int page_validate(const fgw_page_params& p, int op);

@@ -369,6 +369,13 @@ FGW_API int fgw_chunk_workspace_size(const fgw_chunk_params* params, size_t* byt
 /* `workspace` must be 256-byte aligned device memory; fgw_mha_read_error reads its device-side status. */
 FGW_API int fgw_chunk_attention(const fgw_chunk_params* params, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Self-test of fgw_chunk_attention's failure detection: the same call, whose loads of K (short_loads = 1), V (2) or both
+ * (3) bring half of the rows that the kernels wait for. Waits run out after wait_budget_ms, and the kernels give up as on
+ * any lost load: they record FGW_ERR_DEVICE_TIMEOUT, let their copies in flight land and return, with no trap or fault.
+ * Every wait is bounded; `out` is then undefined. */
+FGW_API int fgw_chunk_selftest_wait(const fgw_chunk_params* params, int short_loads, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /*
  * Page-table operators. Row b of block_table holds the pages of its first cache_seqlens[b] tokens; a page that no row
  * holds is free. Entries of table_out past a row's pages are -1. Page ids outside [0, num_pages) are passed on and
