@@ -23,6 +23,15 @@ TOKENS = [
     ([2] * 6, [500 + 100 * i for i in range(6)], 8, 1, 176, 16, True),
 ]
 
+# chunks (tensor kernel), and chunks among single tokens (both kernels): items cut, whole, of one tile and two
+CHUNKS = [
+    ([600], [1600], 8, 2, 128, 64, True),
+    ([70, 1, 300, 128, 1], [170, 3000, 310, 128, 700], 16, 16, 128, 128, True),
+    ([400, 30, 1, 130, 257, 1], [500, 3000, 1200, 130, 2000, 1], 24, 8, 64, 32, True),
+    ([100, 33, 1, 200], [1100, 33, 400, 600], 6, 2, 176, 48, True),
+    ([140, 1, 90], [300, 2000, 1000], 4, 2, 256, 64, False),
+]
+
 
 def native_call(case, dtype=torch.bfloat16, budget_ms=20):
     """(params, workspace, guarded output, inputs) of one call by the C ABI."""
@@ -67,6 +76,12 @@ def run_case(case, short, sites):
 @pytest.mark.parametrize("case", TOKENS, ids=range(len(TOKENS)))
 def test_decode_kernel_gives_up_on_lost_loads(case, short):
     run_case(case, short, sites=(70, 71))
+
+
+@pytest.mark.parametrize("short", [1, 2, 3])
+@pytest.mark.parametrize("case", CHUNKS, ids=range(len(CHUNKS)))
+def test_tensor_kernel_gives_up_on_lost_loads(case, short):
+    run_case(case, short, sites=(70, 71, *range(80, 94)))
 
 
 def test_selftest_refuses():
