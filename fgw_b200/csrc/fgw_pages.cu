@@ -30,6 +30,8 @@ constexpr int kPlanCtas = 8;       // one portable cluster
 constexpr int kPlanThreads = 1024;
 constexpr int kSmallPages = 1 << 17, kSmallRows = 4096, kSmallEntries = 1 << 15;  // one CTA's share
 constexpr int kPlanLoads = 4;
+// The plan's loops count entries and rows in 32 bits and step by up to all threads' loads past the last one.
+static_assert(FGW_PAGE_MAX_ENTRIES + 1ll * kPlanCtas * kPlanThreads * kPlanLoads <= 0x7fffffffll, "loops over a table");
 constexpr int kBlockWords = 32;    // bitmap words ranked together by one warp (1024 pages)
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 8;  // 32 KB of a page per step: 257 us against 263 with 16 KB (1.47 GB moved)
@@ -473,7 +475,7 @@ int page_validate(const fgw_page_params& p, int op) {
   }
   if (p.batch <= 0 || p.table_width <= 0) return FGW_ERR_INVALID_ARGUMENT;
   if (static_cast<long long>(p.page_size) * p.table_width > 0x7fffffffll) return FGW_ERR_INVALID_ARGUMENT;
-  if (static_cast<long long>(p.batch) * p.table_width > 0x7fffffffll) return FGW_ERR_INVALID_ARGUMENT;
+  if (static_cast<long long>(p.batch) * p.table_width > FGW_PAGE_MAX_ENTRIES) return FGW_ERR_INVALID_ARGUMENT;
   if (p.block_table == nullptr || p.cache_seqlens == nullptr || p.table_out == nullptr || p.status == nullptr ||
       p.table_out == p.block_table) {
     return FGW_ERR_INVALID_ARGUMENT;

@@ -236,8 +236,8 @@ void check_table(const at::Tensor& table, const at::Tensor& lens, int64_t page, 
                  fgw_page_params& p) {
   require(table.dim() == 2 && lens.dim() == 1 && lens.size(0) == table.size(0) && table.numel() > 0,
           "metadata shape mismatch");
-  require(table.size(1) <= kInt32Max / page && table.numel() <= kInt32Max,
-          "requires logical positions and table entries to fit int32");
+  require(table.size(1) <= kInt32Max / page && table.numel() <= FGW_PAGE_MAX_ENTRIES,
+          "requires logical positions to fit int32 and at most 2^31 - 2^16 table entries");
   check_rows(table, pool);
   check_rows(lens, pool);
   p.block_table = ints(table);

@@ -382,6 +382,7 @@ FGW_API int fgw_chunk_selftest_wait(const fgw_chunk_params* params, int short_lo
  * never read or written. The pools are the K and V caches of every layer, of one shape: pools[i] is
  * [num_pages * page_size] rows of row_bytes bytes each.
  */
+#define FGW_PAGE_MAX_ENTRIES 0x7fff0000ll /* largest batch * table_width, 2^31 - 2^16 */
 typedef struct fgw_page_params {
   void* const* pools;           /* [pool_count] device pointers, in host memory; 16-byte aligned */
   const int32_t* block_table;   /* [batch, table_width] */
