@@ -502,10 +502,10 @@ cudaError_t launch_chunk(const fgw_chunk_params& p, int short_boxes, void* works
   MergeArgs merge = {};
   merge.ws = static_cast<WorkspaceHeader*>(workspace);
   for (int k = 0; k < 2; ++k) {
+    if (!on[k]) continue;  // a decode item holds no token of more than 64 heads per key head
     a[k].tokens_per_item = layout.tokens_per_item[k];
     a[k].by_item_tokens = FastDiv(layout.tokens_per_item[k]);
     a[k].slots = layout.slots[k];
-    if (!on[k]) continue;
     merge.list[k].slots = layout.slots[k];
     merge.list[k].slot_rows = layout.slot_rows[k];
     merge.list[k].rows = kMergeRows[k];

@@ -2,6 +2,7 @@
 // requests end to end, cu[b] <= t < cu[b + 1] for request b's rows).
 #pragma once
 
+#include <assert.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -16,6 +17,7 @@ struct FastDiv {
   int by;
   FastDiv() = default;
   explicit FastDiv(int d) : by(d) {
+    assert(d > 0);
     uint32_t l = 0;
     while (l < 31 && (1u << l) < static_cast<uint32_t>(d)) ++l;
     mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - d)) / d + 1);

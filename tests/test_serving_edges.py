@@ -2,6 +2,7 @@
 are not finite. Exact where integers are compared; tolerances elsewhere are those of test_serving_ops.py.
 """
 import ctypes
+import subprocess
 
 import pytest
 import torch
@@ -41,3 +42,59 @@ def test_page_operators_refuse_tables_past_their_loops_from_python():
         fork_pages(pool, table, lens, lens, 1)
     with pytest.raises(ValueError, match="table entries"):
         compact_pages(pool, table, lens, 1)
+
+
+HOST_DRIVER = r"""
+#include "fgw_chunk.cuh"
+
+namespace fgw {  // what the host side calls on its way; nothing is launched
+cudaError_t prepare_kernel(const void*, int, int, int*) { return cudaErrorNotSupported; }
+CUresult encode_tiled_cached(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill) {
+  return CUDA_ERROR_NOT_SUPPORTED;
+}
+cudaError_t launch_chunk_decode(const fgw_chunk_params&, ChunkArgs, int, cudaStream_t) { return cudaErrorNotSupported; }
+cudaError_t launch_chunk_tensor(const fgw_chunk_params&, ChunkArgs, const ChunkList&, int, cudaStream_t) {
+  return cudaErrorNotSupported;
+}
+}  // namespace fgw
+
+int main() {
+  for (int group = 1; group <= fgw::kMaxGroup; ++group) {
+    for (int tokens = 1; tokens <= 300; tokens += 13) {
+      for (int dim = 64; dim <= 256; dim += 64) {
+        fgw_chunk_params p = {};
+        p.tokens = tokens;
+        p.batch = 3;
+        p.heads = group;
+        p.kv_heads = 1;
+        p.head_dim = dim;
+        p.page_size = p.pool_rows = 16;
+        p.table_width = 1;
+        p.q_stride = p.out_stride = group * dim;
+        p.dtype = FGW_DTYPE_BFLOAT16;
+        p.softmax_scale = 1.f;
+        if (fgw::chunk_validate(p) != FGW_OK) return 1;
+        if (fgw::launch_chunk(p, 0, nullptr, 148, 0, nullptr) != cudaErrorNotSupported) return 2;
+      }
+    }
+  }
+  return 0;
+}
+"""
+
+
+def test_the_host_side_of_chunk_attention_is_defined_for_every_group(tmp_path):
+    """The host code for up to 128 heads per key head, unoptimised and checked: no division by zero, no overflow."""
+    from fgw_b200 import build
+    driver = tmp_path / "driver.cu"
+    driver.write_text(HOST_DRIVER)
+    checks = "-fsanitize=undefined,-fno-sanitize-recover=all"
+    command = [build.nvcc(), *build.ARCH, "-std=c++17", "-O0", "-Xcompiler", checks, "--expt-relaxed-constexpr",
+               f"-I{build.INCLUDE}", f"-I{build.CSRC}", str(driver), str(build.CSRC / "fgw_chunk.cu"), "-o",
+               str(tmp_path / "driver")]
+    made = subprocess.run(command, capture_output=True, text=True)
+    assert made.returncode == 0, made.stderr
+    ran = subprocess.run([str(tmp_path / "driver")], capture_output=True, text=True)
+    assert ran.returncode == 0, (ran.returncode, ran.stderr)
