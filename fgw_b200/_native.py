@@ -64,6 +64,7 @@ EXPORTED = (
     "fgw_rotary_append",
     "fgw_chunk_workspace_size",
     "fgw_chunk_attention",
+    "fgw_chunk_read_error",
     "fgw_chunk_selftest_wait",
     "fgw_page_workspace_size",
     "fgw_page_fork",
@@ -272,6 +273,8 @@ def library():
         fn = getattr(lib, name)
         fn.argtypes = [vp, ctypes.POINTER(ctypes.c_size_t)]
         fn.restype = ctypes.c_int
+    lib.fgw_chunk_read_error.argtypes = [vp, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]
+    lib.fgw_chunk_read_error.restype = ctypes.c_int
     lib.fgw_chunk_selftest_wait.argtypes = [vp, ctypes.c_int, vp, ctypes.c_size_t, vp]
     lib.fgw_chunk_selftest_wait.restype = ctypes.c_int
     for name in ("fgw_chunk_attention", "fgw_page_fork", "fgw_page_compact", "fgw_page_copy"):
@@ -388,6 +391,14 @@ def static_ws_read_error(stream_ptr):
     site = ctypes.c_int(0)
     check(library().fgw_mha_static_ws_read_error(stream_ptr, ctypes.byref(status), ctypes.byref(site)),
           "fgw_mha_static_ws_read_error")
+    return status.value, site.value
+
+
+def chunk_read_error(stream_ptr):
+    """(device_status, site) of the chunk-attention calls on the current device since the last report; synchronises."""
+    status, site = ctypes.c_int(0), ctypes.c_int(0)
+    check(library().fgw_chunk_read_error(ctypes.c_void_p(stream_ptr), ctypes.byref(status), ctypes.byref(site)),
+          "fgw_chunk_read_error")
     return status.value, site.value
 
 

@@ -514,6 +514,18 @@ int fgw_chunk_selftest_wait(const fgw_chunk_params* params, int short_loads, voi
   return chunk_attention(params, short_loads, workspace, workspace_bytes, stream);
 }
 
+int fgw_chunk_read_error(void* stream, int* device_status, int* site) {
+  if (device_status == nullptr) return FGW_ERR_INVALID_ARGUMENT;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return FGW_ERR_NO_DEVICE;
+  if (cudaStreamSynchronize(static_cast<cudaStream_t>(stream)) != cudaSuccess) return FGW_ERR_CUDA;
+  int words[2] = {0, 0};
+  if (take_chunk_error(words) != cudaSuccess) return FGW_ERR_CUDA;
+  *device_status = words[0];
+  if (site != nullptr) *site = words[1];
+  return FGW_OK;
+}
+
 static int page_workspace_size(const fgw_page_params* params, int op, size_t* bytes) {
   if (params == nullptr || bytes == nullptr) return FGW_ERR_INVALID_ARGUMENT;
   if (params->batch < 0 || params->num_pages <= 0 || params->num_pages > (1 << 30) || params->copy_count < 0) {

@@ -242,6 +242,10 @@ struct MergeArgs {
   MergeList list[2];  // decode, tensor; parts 0: kernel not launched
 };
 
+// The first error of the calls on this device since it was last read {fgw_status, wait site}: a caller whose workspace is
+// gone when the call returns has no other place to look.
+__device__ int g_chunk_error[2];
+
 __device__ void merge_errors(const MergeArgs& m) {
   int code = 0, site = 0;
   for (int k = 0; k < 2; ++k) {
@@ -260,6 +264,7 @@ __device__ void merge_errors(const MergeArgs& m) {
   if (threadIdx.x == 0) {
     m.ws->error = code;
     m.ws->error_site = site;
+    if (code != 0 && atomicCAS(&g_chunk_error[0], 0, code) == 0) g_chunk_error[1] = site;
   }
 }
 
@@ -345,6 +350,13 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
     reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + t * a.out_stride)[i % chunks] = make_uint4(0, 0, 0, 0);
   }
   if (blockIdx.x == 0 && tid < 32) merge_errors(m);
+}
+
+cudaError_t take_chunk_error(int (&words)[2]) {
+  const cudaError_t err = cudaMemcpyFromSymbol(words, g_chunk_error, sizeof(words), 0, cudaMemcpyDeviceToHost);
+  if (err != cudaSuccess || words[0] == 0) return err;
+  const int none[2] = {0, 0};
+  return cudaMemcpyToSymbol(g_chunk_error, none, sizeof(none), 0, cudaMemcpyHostToDevice);
 }
 
 int chunk_validate(const fgw_chunk_params& p) {

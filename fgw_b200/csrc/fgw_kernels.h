@@ -110,6 +110,7 @@ int chunk_validate_pointers(const fgw_chunk_params& p);
 size_t chunk_workspace_bytes(const fgw_chunk_params& p);
 cudaError_t launch_chunk(const fgw_chunk_params& p, int short_boxes, void* workspace, int sm_count, int device,
                          cudaStream_t stream);
+cudaError_t take_chunk_error(int (&words)[2]);  // {status, site} kept on the current device, which is cleared
 // Page-table operators (fgw_pages.cu).
 enum PageOp { kPageFork = 0, kPageCompact = 1, kPageCopy = 2 };
 int page_validate(const fgw_page_params& p, int op);

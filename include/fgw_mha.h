@@ -369,6 +369,11 @@ FGW_API int fgw_chunk_workspace_size(const fgw_chunk_params* params, size_t* byt
 /* `workspace` must be 256-byte aligned device memory; fgw_mha_read_error reads its device-side status. */
 FGW_API int fgw_chunk_attention(const fgw_chunk_params* params, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Device-side status for callers that do not keep the workspace (the Python entry point): synchronises `stream`, then
+ * reports the first error that calls on the current device recorded since the last report (FGW_OK when there was none) and
+ * which wait site gave up, and clears it. After an error the outputs of that call are undefined. */
+FGW_API int fgw_chunk_read_error(void* stream, int* device_status, int* site);
+
 /* Self-test of fgw_chunk_attention's failure detection: the same call, whose loads of K (short_loads = 1), V (2) or both
  * (3) bring half of the rows that the kernels wait for. Waits run out after wait_budget_ms, and the kernels give up as on
  * any lost load: they record FGW_ERR_DEVICE_TIMEOUT, let their copies in flight land and return, with no trap or fault.

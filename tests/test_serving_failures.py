@@ -89,3 +89,23 @@ def test_selftest_refuses():
     for short in (-1, 4):
         assert _native.library().fgw_chunk_selftest_wait(ctypes.byref(p), short, workspace.data_ptr(), workspace.numel(),
                                                          None) == 1
+
+
+def test_a_lost_load_is_reported_to_python_once():
+    """The Python call's workspace is gone when it returns: the status stays readable, for each device, until it is read."""
+    from fgw_b200.operators.mha.chunk_attention import paged_chunk_attention, read_error
+    lib, stream = _native.library(), torch.cuda.current_stream().cuda_stream
+    read_error()
+    for case in (TOKENS[2], CHUNKS[2]):
+        p, workspace, room, inputs, gpu = native_call(case)
+        args = (workspace.data_ptr(), workspace.numel(), stream)
+        assert lib.fgw_chunk_selftest_wait(ctypes.byref(p), 1, *args) == 0
+        first = _native.read_error(workspace.data_ptr(), stream)
+        assert lib.fgw_chunk_attention(ctypes.byref(p), *args) == 0  # a later good call does not cover it
+        new, held, heads, kv_heads, dim, page, causal = case
+        paged_chunk_attention(*gpu, page, is_causal=causal)
+        assert first[0] == _native.ERR_DEVICE_TIMEOUT
+        assert read_error() == first
+        assert read_error(0) == (_native.OK, 0)
+        check_attention(paged_chunk_attention(*gpu, page, is_causal=causal), *inputs, page, causal, dim ** -0.5)
+        assert read_error(torch.device("cuda", 0)) == (_native.OK, 0)
