@@ -41,16 +41,18 @@ struct PageCopy {
   int32_t src, dst, rows;  // rows: token rows of the page to copy; <= 0 skips the entry
 };
 
-// Workspace: copy list | copy count and totals | bitmap | per-block ranks | free list | row arrays.
+// Workspace: copy count and totals | copy list | bitmaps | per-block ranks | free list | row arrays.
 struct PageWs {
   PageCopy* copies;
   int32_t* totals;   // [0] copies, [1] needed pages, [2] free pages, [3] moved pages
-  uint32_t* used;    // bitmap of the held pages
+  uint32_t* used;    // bitmap of the held pages; fork: of those that hold a row's partly filled end
+  uint32_t* shut;    // fork: bitmap of the pages that no row may keep as its partly filled end
   int32_t* blocks;   // free pages before each block of 1024 pages, exclusive
   int32_t* list;     // fork: free pages in order; compact: holes, moved pages (last first), then new ids by page
   int32_t* first;    // [batch] first row with this parent
   int32_t* need;     // [batch + 1] new pages of each row, then their exclusive prefix
-  int4* rows;        // [batch] what each row becomes: {parent, entries kept, entries wanted, entries held}
+  int4* rows;        // [batch] what each row becomes: {parent, entries kept, entries wanted, entries held}; until the
+                     // copies are known, fork's entries kept are the full ones
 };
 
 struct PageArgs {
@@ -82,6 +84,7 @@ static size_t carve_pages(const fgw_page_params& p, void* base, PageWs* ws) {
   w.totals = reinterpret_cast<int32_t*>(take(64));
   w.copies = reinterpret_cast<PageCopy*>(take(copies * sizeof(PageCopy)));
   w.used = reinterpret_cast<uint32_t*>(take(blocks * kBlockWords * 4));
+  w.shut = reinterpret_cast<uint32_t*>(take(blocks * kBlockWords * 4));
   w.blocks = reinterpret_cast<int32_t*>(take((blocks + 1) * 4));
   w.list = reinterpret_cast<int32_t*>(take(3 * static_cast<size_t>(p.num_pages) * 4));
   w.first = reinterpret_cast<int32_t*>(take(static_cast<size_t>(p.batch) * 4));
@@ -149,6 +152,7 @@ __device__ int cta_exclusive_scan(int32_t* x, int n, int* shared, Load load) {
 struct SmallWs {
   int32_t totals[4];
   uint32_t used[kSmallPages / 32];
+  uint32_t shut[kSmallPages / 32];
   int32_t blocks[kSmallPages / (32 * kBlockWords) + 1];
   int32_t first[kSmallRows];
   int32_t need[kSmallRows + 1];
@@ -161,6 +165,7 @@ __device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
   if constexpr (kCtas == 1) {
     SmallWs& small = *reinterpret_cast<SmallWs*>(plan_smem);
     a.ws.used = small.used;
+    a.ws.shut = small.shut;
     a.ws.blocks = small.blocks;
     a.ws.first = small.first;
     a.ws.need = small.need;
@@ -195,13 +200,14 @@ __device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
     uint32_t bits = 0;
     if (first_page + 32 > a.pages) bits = first_page >= a.pages ? 0xffffffffu : 0xffffffffu << (a.pages & 31);
     a.ws.used[w] = bits;
+    if (kFork) a.ws.shut[w] = 0;
   }
   if (tid < 4) totals[tid] = 0;
   for (int i = tid; i < a.batch; i += kThreads) {
     if (kFork) {
       a.ws.first[i] = a.batch;
       const ForkRow r = fork_row(a, i);
-      a.ws.rows[i] = make_int4(r.parent, r.held, r.want, r.held);
+      a.ws.rows[i] = make_int4(r.parent, r.full, r.want, r.held);
     } else {
       const int len = clamped_len(a, a.lens[i]);
       a.ws.rows[i] = make_int4(i, 0, 0, len / a.page + (len % a.page != 0));
@@ -216,10 +222,12 @@ __device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
     sync();
   }
   // The held pages; of the rows with one parent only the first marks. Table entries are taken flat, four loads of a
-  // thread at a time.
+  // thread at a time. A partly filled end may stay with its row only if no other parent's row, and no other entry of its
+  // own, holds that page: full pages shut it, and so does the second end on one page, whichever of them comes second.
   const int entries = a.batch * a.width;
   for (int base = tid; base < entries; base += kThreads * kPlanLoads) {
     int ids[kPlanLoads];
+    bool full[kPlanLoads];  // fork: a full page's entry
 #pragma unroll
     for (int u = 0; u < kPlanLoads; ++u) {
       ids[u] = -1;
@@ -229,23 +237,41 @@ __device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
       const int parent = fresh(&a.ws.rows[i].x), held = fresh(&a.ws.rows[i].w);
       if (w >= held || (kFork && fresh(&a.ws.first[parent]) != i)) continue;  // held is 0 without a parent
       ids[u] = a.table[static_cast<long long>(parent) * a.width + w];
+      full[u] = kFork && w < fresh(&a.ws.rows[i].y);
     }
 #pragma unroll
     for (int u = 0; u < kPlanLoads; ++u) {
-      if (ids[u] >= 0 && ids[u] < a.pages) atomicOr(&a.ws.used[ids[u] >> 5], 1u << (ids[u] & 31));
-    }
-  }
-  if (kFork) {
-    for (int i = tid; i < a.batch; i += kThreads) {
-      const ForkRow r = fork_row(a, i);
-      const bool copies = r.parent >= 0 && r.len > r.full * a.page && fresh(&a.ws.first[r.parent]) != i;
-      a.ws.need[i] = (copies ? 1 : 0) + r.want - r.held;
-      if (copies) a.ws.rows[i].y = r.full;
+      if (ids[u] < 0 || ids[u] >= a.pages) continue;
+      const int word = ids[u] >> 5;
+      const uint32_t bit = 1u << (ids[u] & 31);
+      if (!kFork) {
+        atomicOr(&a.ws.used[word], bit);
+      } else if (full[u] || (atomicOr(&a.ws.used[word], bit) & bit) != 0) {
+        atomicOr(&a.ws.shut[word], bit);
+      }
     }
   }
   sync();
+  auto held_pages = [&](int word) {
+    uint32_t bits = fresh(&a.ws.used[word]);
+    if (kFork) bits |= fresh(&a.ws.shut[word]);
+    return bits;
+  };
+  if (kFork) {
+    for (int i = tid; i < a.batch; i += kThreads) {
+      const ForkRow r = fork_row(a, i);
+      bool copies = false;
+      if (r.held > r.full) {
+        const int end = a.table[static_cast<long long>(r.parent) * a.width + r.full];
+        copies = fresh(&a.ws.first[r.parent]) != i ||
+                 (end >= 0 && end < a.pages && (fresh(&a.ws.shut[end >> 5]) >> (end & 31) & 1) != 0);
+      }
+      a.ws.need[i] = (copies ? 1 : 0) + r.want - r.held;
+      if (!copies) a.ws.rows[i].y = r.held;
+    }
+  }
   for (int b = warp; b < a.blocks; b += kWarps) {
-    const int free_here = 32 - __popc(fresh(&a.ws.used[b * kBlockWords + lane]));
+    const int free_here = 32 - __popc(held_pages(b * kBlockWords + lane));
     const int sum = __reduce_add_sync(0xffffffffu, free_here);
     if (lane == 0) a.ws.blocks[b] = sum;
   }
@@ -268,7 +294,7 @@ __device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
     int rank = fresh(&a.ws.blocks[b]);
     if (kFork && rank >= needed) continue;
     const int w = b * kBlockWords + lane;
-    const uint32_t used = fresh(&a.ws.used[w]);
+    const uint32_t used = held_pages(w);
     const int free_here = 32 - __popc(used);
     int sum = free_here;
 #pragma unroll
@@ -302,7 +328,7 @@ __device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
     for (int i = tid; i < a.batch; i += kThreads) {
       const ForkRow r = fork_row(a, i);
       a.lens_out[i] = fits ? r.len : a.lens[i];
-      if (!fits || r.parent < 0 || r.len <= r.full * a.page || fresh(&a.ws.first[r.parent]) == i) continue;
+      if (!fits || r.held == r.full || fresh(&a.ws.rows[i].y) == r.held) continue;  // nothing to copy
       const int src = a.table[static_cast<long long>(r.parent) * a.width + r.full];
       const int dst = __ldcg(&a.ws.list[fresh(&a.ws.need[i])]);
       const int at = atomicAdd(&totals[0], 1);

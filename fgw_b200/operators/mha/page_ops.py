@@ -16,10 +16,12 @@ def fork_pages(pools, block_table, cache_seqlens, parents, page_size, reserve_se
 
     ``parents`` [B] int32 reads the rows as they were: a row's own index keeps it, an index outside [0, B) frees it, and
     a beam step's choice is passed as it is. Full pages are shared. A partly filled last page stays with the first row
-    that has its parent; the others get a page of their own with the filled tokens copied in every pool. Then row i has
-    pages for ``reserve_seqlens[i]`` tokens (at least its own; at most the table's width). New pages are the lowest
-    free ones. ``status`` [2] int32 is (pages needed, pages free): when the first is larger, the state is returned as
-    it was and nothing is copied.
+    that has its parent; the others get a page of their own with the filled tokens copied in every pool. So does the first
+    where another parent's row holds that page too, as after a length was lowered: afterwards the page that a row's next
+    token goes to is the row's own (so a lowered row passes through here before it is appended to). Then row i has pages
+    for ``reserve_seqlens[i]`` tokens (at least its own; at most the table's width). New pages are the lowest free ones.
+    ``status`` [2] int32 is (pages needed, pages free): when the first is larger, the state is returned as it was and
+    nothing is copied.
     """
     return _native.torch_binding().fork_pages(pools, block_table, cache_seqlens, parents, page_size, reserve_seqlens)
 

@@ -414,9 +414,11 @@ FGW_API int fgw_page_workspace_size(const fgw_page_params* params, size_t* bytes
 
 /* Every row i becomes a fork of row parents[i] as it was (its own index keeps it; an index outside [0, batch) frees the
  * row): the parent's full pages are shared; its partly filled last page stays with the first row that has this parent
- * and is copied for the others (the filled token rows, in every pool); reserve_seqlens[i] tokens (no fewer than the
- * parent's) get pages. New pages are the lowest free ones, given in (row, column) order. status = {pages needed, pages
- * free}; when more are needed than free, the outputs are the inputs and nothing is copied. */
+ * and is copied for the others (the filled token rows, in every pool). Where another parent's row holds that page too (a
+ * length was lowered), or the parent itself a second time, it is copied for the first row as well: afterwards the page that
+ * a row's next token goes to is that row's alone. reserve_seqlens[i] tokens (no fewer than the parent's) get pages. New
+ * pages are the lowest ones that no parent held, given in (row, column) order. status = {pages needed, pages free}; when
+ * more are needed than free, the outputs are the inputs and nothing is copied. */
 FGW_API int fgw_page_fork(const fgw_page_params* params, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Moves the held pages into the lowest ids: with `live` pages held, the k-th held page from id `live` on goes to the k-th

@@ -61,12 +61,16 @@ def rotary_append(q, k, v, k_cache, v_cache, table, lens, cu, cos_sin, page, int
 
 def fork_pages(table, lens, parents, reserve, page, pages):
     """(table, lens, (needed, free), copies) with copies [(src, dst, filled rows)]; the state as it was when too few
-    pages are free."""
+    pages are free. The first row with a parent keeps its partly filled last page if nothing else holds that page."""
     rows, width = table.shape
     kept = [int(p) if 0 <= p < rows else -1 for p in parents]
     length = [min(max(int(lens[p]), 0), width * page) if p >= 0 else 0 for p in kept]
     held = {int(e) for p, n in zip(kept, length) if p >= 0 for e in table[p, :-(-n // page)] if 0 <= e < pages}
     free = [e for e in range(pages) if e not in held]
+    holds = {}  # page -> places (parent, entry) that hold it
+    for p in set(kept) - {-1}:
+        for w in range(-(-length[kept.index(p)] // page)):
+            holds.setdefault(int(table[p, w]), []).append((p, w))
     out = np.full_like(table, -1)
     needed, copies, seen = 0, [], set()
     for i, (p, n) in enumerate(zip(kept, length)):
@@ -76,7 +80,7 @@ def fork_pages(table, lens, parents, reserve, page, pages):
         have = -(-n // page)
         out[i, :have] = table[p, :have]
         fresh = list(range(have, -(-room // page)))
-        if n % page and p in seen:
+        if n % page and (p in seen or 0 <= table[p, have - 1] < pages and len(holds[int(table[p, have - 1])]) > 1):
             fresh.insert(0, have - 1)
         for w in fresh:
             new = free[needed] if needed < len(free) else -1

@@ -4,10 +4,13 @@ are not finite. Exact where integers are compared; tolerances elsewhere are thos
 import ctypes
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
 from fgw_b200 import _native
+from oracle import serving
+from test_serving_ops import on_gpu, values
 
 MAX_ENTRIES = 2 ** 31 - 2 ** 16
 
@@ -98,3 +101,63 @@ def test_the_host_side_of_chunk_attention_is_defined_for_every_group(tmp_path):
     assert made.returncode == 0, made.stderr
     ran = subprocess.run([str(tmp_path / "driver")], capture_output=True, text=True)
     assert ran.returncode == 0, (ran.returncode, ran.stderr)
+
+
+# --- pages that several rows hold -----------------------------------------------------------------------------------
+# (name, pages of each row, held, parents, reserve, spare pages); pages of 16 tokens. Rows come to hold the same partly
+# filled page when a length is lowered, as for a cached prefix of which only a part fits the new text.
+SHARED = [
+    ("part_of_a_prefix", [[3, 5, 7], [3, 5, 7]], [48, 40], [0, 1], None, 4),
+    ("part_of_a_prefix_forked", [[3, 5, 7], [3, 5, 7], []], [48, 40, 0], [1, 0, 1], [41, 48, 41], 4),
+    ("inner_page", [[3, 5, 7], [3, 5]], [48, 20], [0, 1], [49, 21], 4),
+    ("two_parts", [[3, 5], [3, 5]], [20, 30], [0, 1], [21, 31], 4),
+    ("three_parts", [[3, 5], [3, 5], [3, 5]], [20, 30, 17], [2, 1, 0], None, 4),
+    ("forks_of_two_parts", [[3, 5], [3, 5], [], []], [20, 30, 0, 0], [0, 1, 0, 1], [33, 31, 21, 31], 9),
+    ("the_other_leaves", [[3, 5, 7], [3, 5, 7]], [48, 40], [-1, 1], [0, 41], 4),
+    ("whole_pages_stay_shared", [[3, 5, 7], [3, 5, 7]], [48, 32], [0, 1], [49, 33], 4),
+    ("twice_in_a_row", [[3, 3]], [20], [0], [21], 4),
+    ("too_few_for_the_copy", [[0, 1, 2], [0, 1, 2]], [48, 40], [0, 1], None, 0),
+    ("empty", [[3, 5], [3, 5]], [0, 20], [0, 1], [1, 21], 4),
+]
+
+
+def shared_state(rows, held, spare):
+    width = max(max(map(len, rows)), 1) + 3
+    table = np.full((len(rows), width), -1, dtype=np.int32)
+    for b, row in enumerate(rows):
+        table[b, :len(row)] = row
+    return table, np.array(held, dtype=np.int32), int(table.max()) + 1 + spare
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SHARED, ids=[c[0] for c in SHARED])
+def test_fork_copies_a_partly_filled_page_that_another_row_holds(case):
+    """After a fork the page that a row's next token goes to is the row's own."""
+    from fgw_b200.operators.mha.page_ops import fork_pages
+    name, rows, held, parents, reserve, spare = case
+    page = 16
+    table, lens, pages = shared_state(rows, held, spare)
+    parents = np.array(parents, dtype=np.int32)
+    reserve = None if reserve is None else np.array(reserve, dtype=np.int32)
+    want_table, want_lens, want_status, copies = serving.fork_pages(table, lens, parents, reserve, page, pages)
+    store = values((pages * page, 2, 16), torch.bfloat16, 3)
+    pool = store.cuda()
+    got = fork_pages([pool], *on_gpu(table, lens, parents), page,
+                     reserve_seqlens=None if reserve is None else on_gpu(reserve)[0])
+    assert tuple(got[2].tolist()) == want_status
+    assert np.array_equal(got[0].cpu().numpy(), want_table)
+    assert np.array_equal(got[1].cpu().numpy(), want_lens)
+    assert torch.equal(pool.cpu().view(torch.int16),
+                       torch.from_numpy(serving.copy_rows(store.view(torch.int16).numpy(), copies, page)))
+    if want_status[0] > want_status[1]:
+        return
+    table2, lens2 = got[0].cpu().numpy(), got[1].cpu().numpy()
+    entries = [table2[b, :-(-n // page)].tolist() for b, n in enumerate(lens2)]
+    for b, n in enumerate(lens2):
+        if n % page:
+            assert sum(row.count(entries[b][-1]) for row in entries) == 1, (b, entries)
+        # and the row still has its parent's tokens
+        if parents[b] >= 0:
+            before = [int(table[parents[b], t // page]) * page + t % page for t in range(n)]
+            after = [entries[b][t // page] * page + t % page for t in range(n)]
+            assert torch.equal(pool[after].cpu(), store[before])
