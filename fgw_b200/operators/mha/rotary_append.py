@@ -50,7 +50,8 @@ def rotary_table(positions, rotary_dim, base=10000.0, scaling=None, factor=1.0, 
             return pairs * math.log(original_positions / (turns * 2.0 * math.pi)) / math.log(base)
 
         low = max(math.floor(pair_of(beta_fast)), 0)
-        high = min(math.ceil(pair_of(beta_slow)), pairs - 1)
+        # may lie past the last pair, whose blend then ends unfinished; the limit is the published one
+        high = min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
         slow = ((index - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
         freq = freq * (1.0 - slow) + freq / factor * slow
         size = 0.1 * math.log(factor) + 1.0 if attention_factor is None else float(attention_factor)

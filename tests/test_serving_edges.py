@@ -2,6 +2,7 @@
 are not finite. Exact where integers are compared; tolerances elsewhere are those of test_serving_ops.py.
 """
 import ctypes
+import math
 import subprocess
 
 import numpy as np
@@ -161,3 +162,29 @@ def test_fork_copies_a_partly_filled_page_that_another_row_holds(case):
             before = [int(table[parents[b], t // page]) * page + t % page for t in range(n)]
             after = [entries[b][t // page] * page + t % page for t in range(n)]
             assert torch.equal(pool[after].cpu(), store[before])
+
+
+# --- YaRN angles ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("base,dim,trained,factor", [
+    (10000.0, 128, 131072, 4.0), (10000.0, 128, 4096, 16.0), (500.0, 64, 8192, 8.0), (1e6, 96, 32768, 2.0),
+    (10000.0, 32, 100, 4.0),
+])
+def test_yarn_blends_by_the_turns_of_every_pair(base, dim, trained, factor):
+    """Every pair, the middle of the blend and pairs past which it would run included, against the published ramp: over the
+    pair index from floor(pair of beta_fast turns), at least 0, to ceil(pair of beta_slow turns), at most dim - 1."""
+    from fgw_b200.operators.mha.rotary_append import rotary_table
+    got = rotary_table(2, dim, base=base, scaling="yarn", factor=factor, original_positions=trained, attention_factor=1.0,
+                       device="cpu").double()
+    low = max(math.floor(dim * math.log(trained / (32.0 * 2 * math.pi)) / (2 * math.log(base))), 0)
+    high = min(math.ceil(dim * math.log(trained / (1.0 * 2 * math.pi)) / (2 * math.log(base))), dim - 1)
+    partly = 0
+    for pair in range(dim // 2):
+        plain = base ** (-2.0 * pair / dim)
+        slow = min(max((pair - low) / max(high - low, 1e-3), 0.0), 1.0)
+        partly += 0.0 < slow < 1.0
+        freq = plain * (1.0 - slow) + plain / factor * slow
+        assert abs(got[1, pair] - math.cos(freq)) <= 2.0 ** -24 + 1e-12  # one rounding to FP32
+        assert abs(got[1, dim // 2 + pair] - math.sin(freq)) <= 2.0 ** -24 + 1e-12
+        if trained * plain / (2 * math.pi) > 1.0 + 1e-6:  # more than beta_slow turns: not fully divided
+            assert slow < 1.0
+    assert partly > 3
