@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
         peak = next;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          const float wk = w[u] > kValidLse ? fast_exp2(w[u] - peak) : 0.f;
+          const float wk = w[u] <= kValidLse ? 0.f : fast_exp2(w[u] - peak);  // a piece's NaN stays one
           sum += wk;
           acc.x = fmaf(wk, v[u].x, acc.x);
           acc.y = fmaf(wk, v[u].y, acc.y);
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
           acc.w = fmaf(wk, v[u].w, acc.w);
         }
       }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       T* out = static_cast<T*>(a.out) + (cut.token0 + token) * a.out_stride +
                static_cast<long long>(cut.hk * a.group + in_tile - in_token * a.group) * a.dim + g * 4;
       *reinterpret_cast<uint2*>(out) =

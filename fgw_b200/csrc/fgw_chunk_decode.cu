@@ -486,7 +486,8 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
         const float4 t0 = *reinterpret_cast<const float4*>(&row_max[r * NW]);
         const float4 t1 = *reinterpret_cast<const float4*>(&row_max[r * NW + 4]);
         const float total = ((t0.x + t0.y) + (t0.z + t0.w)) + ((t1.x + t1.y) + (t1.z + t1.w));
-        const float inv = total > 0.f ? 1.f / total : 0.f;
+        const bool none = total == 0.f;  // no key seen: zeros; a NaN among the scores stays one
+        const float inv = 1.f / total;
         if (sg.slot < 0) {
           if (out_at[mt][u] < 0) continue;
           T* out = static_cast<T*>(a.out) + out_at[mt][u];
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
           for (int i = 0; i < NB; ++i) {
             const int at = (warp * NB + i) * 8;
             if (at >= a.dim) continue;
-            const float x = total > 0.f ? o[mt][i][2 * u] * inv : 0.f, y = total > 0.f ? o[mt][i][2 * u + 1] * inv : 0.f;
+            const float x = none ? 0.f : o[mt][i][2 * u] * inv, y = none ? 0.f : o[mt][i][2 * u + 1] * inv;
             *reinterpret_cast<uint32_t*>(out + at + c2) = Tr::pack2(x, y);
           }
         } else {
@@ -504,10 +505,10 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
           for (int i = 0; i < NB; ++i) {
             const int at = (warp * NB + i) * 8;
             if (at >= a.dim) continue;
-            const float x = total > 0.f ? o[mt][i][2 * u] * inv : 0.f, y = total > 0.f ? o[mt][i][2 * u + 1] * inv : 0.f;
+            const float x = none ? 0.f : o[mt][i][2 * u] * inv, y = none ? 0.f : o[mt][i][2 * u + 1] * inv;
             *reinterpret_cast<float2*>(a.slots.o + at_row * a.dim + at + c2) = make_float2(x, y);
           }
-          if (warp == 0 && lane % 4 == 0) a.slots.lse[at_row] = total > 0.f ? m[mt][u] + fast_log2(total) : kEmptyLse;
+          if (warp == 0 && lane % 4 == 0) a.slots.lse[at_row] = none ? kEmptyLse : m[mt][u] + fast_log2(total);
         }
       }
     }

@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
           l = h == 0 ? l + ld_shared(other_max + next) : ld_shared(other_max + next) + l;
           named_barrier_sync(pair_barrier, 64);  // read by both before the next exchange
         }
-        inv = l > 0.f ? 1.f / l : 0.f;
+        inv = 1.f / l;
         if (ok) tc_fence_after_sync();
       }
       const int row_token = a.by_group.quotient(row), row_head = row - row_token * a.group;
@@ -630,8 +630,9 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
           uint32_t r[16];
           tmem_ld16(o_addr + cb * 16, r);
           tmem_wait_ld();
+          // no key seen: exact zeros; a NaN among the scores stays one
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = l > 0.f ? __uint_as_float(r[i]) * inv : 0.f;  // no key seen: exact zeros
+          for (int i = 0; i < 16; ++i) o[i] = l == 0.f ? 0.f : __uint_as_float(r[i]) * inv;
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = 0.f;
@@ -671,7 +672,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
         }
       }
       if (row_valid && h == 0) {
-        a.slots.lse[static_cast<long long>(sg.slot) * kSlotRows + r] = (n_t > 0 && l > 0.f) ? m + fast_log2(l) : kEmptyLse;
+        a.slots.lse[static_cast<long long>(sg.slot) * kSlotRows + r] = n_t == 0 || l == 0.f ? kEmptyLse : m + fast_log2(l);
       }
       if (n_t > 0) {
         tc_fence_before_sync();

@@ -17,9 +17,10 @@ def paged_chunk_attention(q, k_cache, v_cache, block_table, cache_seqlens, cu_se
     ``q`` is [T, H, D] (each token's heads contiguous, any token stride that is a multiple of 8: a slice of a fused
     projection serves as it is), ``k_cache`` / ``v_cache`` [pool_rows, Hkv, D], ``block_table`` [B, W] int32,
     ``cache_seqlens`` [B] int32 (tokens in the cache with the new ones), ``cu_seqlens_q`` [B + 1] int32. Causal: the
-    i-th of a request's n new tokens sees the first ``cache_seqlens - n + i + 1`` cached ones. Rows that see nothing and
-    rows of no request are exact zeros. ``softmax_scale`` defaults to 1 / sqrt(D). At most
-    128 query heads may share a key head. Raises ValueError for tensors that do not fit this, before any launch. Waits on
+    i-th of a request's n new tokens sees the first ``cache_seqlens - n + i + 1`` cached ones. Rows that see nothing (or
+    only scores of -inf) and rows of no request are exact zeros; a score that is NaN or +inf makes its row NaN. Cached
+    values have to be finite: one that is not reaches rows of its request whose mask hides it too. ``softmax_scale``
+    defaults to 1 / sqrt(D). At most 128 query heads may share a key head. Raises ValueError for tensors that do not fit this, before any launch. Waits on
     the device give up after two seconds; ``read_error`` reports it, and the output is then undefined.
     """
     return _native.torch_binding().paged_chunk_attention(q, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens_q,

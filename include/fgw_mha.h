@@ -336,7 +336,9 @@ FGW_API int fgw_rotary_append(const fgw_rotary_params* params, void* stream);
 /*
  * Attention of the new tokens over the cache: query head h of a token reads key head h / (heads / kv_heads). Causal: the
  * i-th of n new tokens sees the first cache_seqlens - n + i + 1 cached tokens; otherwise all of them. Rows that see
- * nothing, and rows of no request, are written as zeros. Page ids are trusted, as in fgw_mha_paged_fwd. Results are the
+ * nothing (or only scores of -inf), and rows of no request, are written as zeros; a score that is NaN or +inf makes its row
+ * NaN. What pages hold past cache_seqlens may be anything; below it V has to be finite, since a weight of zero times an
+ * infinity is NaN also in rows whose causal mask hides it. Page ids are trusted, as in fgw_mha_paged_fwd. Results are the
  * same bits from call to call.
  */
 typedef struct fgw_chunk_params {

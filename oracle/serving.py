@@ -24,6 +24,8 @@ def chunk_attention(q, k_cache, v_cache, table, lens, cu, page, causal, scale):
             for h in range(q.shape[1]):
                 keys, values = k_cache[rows, h // group], v_cache[rows, h // group]
                 s = keys @ q[cu[b] + i, h] * scale
+                if s.max() == -np.inf:  # every weight is zero: as a row that sees nothing
+                    continue
                 p = np.exp(s - s.max())
                 p /= p.sum()
                 out[cu[b] + i, h] = p @ values

@@ -11,7 +11,7 @@ import torch
 
 from fgw_b200 import _native
 from oracle import serving
-from test_serving_ops import on_gpu, values
+from test_serving_ops import attend_case, on_gpu, values
 
 MAX_ENTRIES = 2 ** 31 - 2 ** 16
 
@@ -188,3 +188,40 @@ def test_yarn_blends_by_the_turns_of_every_pair(base, dim, trained, factor):
         if trained * plain / (2 * math.pi) > 1.0 + 1e-6:  # more than beta_slow turns: not fully divided
             assert slow < 1.0
     assert partly > 3
+
+
+# --- scores that are not finite -------------------------------------------------------------------------------------
+NOT_FINITE = [
+    # (name, new, held, heads, kv heads, dim, page, causal): pieces and whole items of both kernels
+    ("tokens", [1] * 9, [5, 300, 64, 1, 2000, 77, 128, 129, 31], 8, 2, 128, 16, True),
+    ("drafts", [7, 3, 5], [400, 90, 5], 8, 1, 256, 16, True),
+    ("chunk", [200], [900], 4, 2, 128, 32, True),
+    ("chunk_narrow", [200, 1, 70], [500, 40, 70], 4, 2, 64, 32, True),
+    ("chunk_wide", [150, 2], [1200, 30], 2, 1, 192, 64, False),
+    ("whole_items", [40 + 7 * i % 60 for i in range(40)], [140 + 211 * i % 700 for i in range(40)], 8, 8, 128, 64, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")], ids=["nan", "inf", "minus_inf"])
+@pytest.mark.parametrize("case", NOT_FINITE, ids=[c[0] for c in NOT_FINITE])
+def test_attention_of_scores_that_are_not_finite(case, bad):
+    """A query or a key that is not finite makes the outputs of the rows that see it what the formula gives (NaN, not
+    zeros, where a score is NaN or +inf; zeros where all are -inf), and leaves all other rows alone."""
+    from fgw_b200.operators.mha.chunk_attention import paged_chunk_attention
+    _, new, held, heads, kv_heads, dim, page, causal = case
+    q, k, v, table, lens, cu = attend_case(case, torch.bfloat16, seed=41)
+    q[len(q) // 2, heads - 1, dim // 3] = bad
+    for b in range(0, len(new), 3):  # a key in the middle, and (where it is a chunk) one among the new tokens
+        for at in {held[b] // 2, held[b] - (new[b] + 1) // 2}:
+            k[int(table[b, at // page]) * page + at % page, 0, 1] = bad
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, spread = serving.chunk_attention(*(x.double().numpy() for x in (q, k, v)), table, lens, cu, page, causal,
+                                               dim ** -0.5)
+    got = paged_chunk_attention(*(x.cuda() for x in (q, k, v)), *on_gpu(table, lens, cu), page, is_causal=causal)
+    got = got.double().cpu().numpy()
+    lost = np.isnan(want)
+    assert lost.any() and not lost.all()
+    assert np.array_equal(np.isnan(got), lost)
+    bound = 2.0 ** -8 * (2 * np.abs(want) + spread) + 2.0 ** -16 * spread + 1e-6
+    assert (np.abs(got - want)[~lost] <= bound[~lost]).all()
