@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kPlanListThreads)
     for (int r = begin + lane; r < end; r += 32) {
       const int t0 = (r - begin) * a.tokens_per_item;
       const int units = item_units<128>(a, count, len, t0);
-      const bool one_tile = a.dim <= 128 && 2 * (count - t0) <= a.tokens_per_item;
+      const bool one_tile = a.dim <= 128 && count - t0 <= a.tokens_per_item / 2;
       raw[r] = make_int4(b, t0, units, units * (one_tile ? kOneTileStepCost : kStepCost) + kItemCost);
     }
   }

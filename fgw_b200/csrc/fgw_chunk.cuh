@@ -89,18 +89,24 @@ __device__ __forceinline__ int held_tokens(const int32_t* lens, int b, int width
   return min(max(lens[b], 0), width * page);
 }
 
+// n / d rounded up, for 0 <= n < 2^31: the sum with d - 1 would pass 31 bits.
+template <int d>
+__device__ __forceinline__ int ceil_div(int n) {
+  return n / d + (n % d != 0);
+}
+
 // Rows of the request's list, 0 when it belongs to the other kernel.
 __device__ __forceinline__ int item_rows(const ChunkArgs& a, int count, bool decode) {
   if (a.split && (count * a.group <= a.small_rows) != decode) return 0;
-  return a.by_item_tokens.quotient(count + a.tokens_per_item - 1);
+  return count > 0 ? a.by_item_tokens.quotient(count - 1) + 1 : 0;
 }
 
 // KV tiles of the item that starts at the request's token t0; one without keys still costs one (zeros to write).
 template <int kKeys>
 __device__ __forceinline__ int item_units(const ChunkArgs& a, int count, int len, int t0) {
-  const int last = min(t0 + a.tokens_per_item, count) - 1;
+  const int last = t0 + min(a.tokens_per_item, count - t0) - 1;
   const int seen = max(a.causal ? len - count + last + 1 : len, 0);
-  return max((seen + kKeys - 1) / kKeys, 1);
+  return max(ceil_div<kKeys>(seen), 1);
 }
 
 // One run of KV tiles of one item processed by this CTA: a whole item, or a piece of one cut between programs.
@@ -126,7 +132,7 @@ __device__ __forceinline__ void make_segment(const ChunkArgs& a, ChunkSegment& s
   s.count = min(a.tokens_per_item, nt.count - t0);
   s.seen0 = a.causal ? len - nt.count + t0 + 1 : len;
   s.limit = max(a.causal ? s.seen0 + s.count - 1 : len, 0);
-  const int tiles = (s.limit + kKeys - 1) / kKeys;
+  const int tiles = ceil_div<kKeys>(s.limit);
   s.n_begin = first;
   s.n = max(0, min(first + count, tiles) - first);
   // a piece that starts inside its item is its program's first, one that starts the item its program's last

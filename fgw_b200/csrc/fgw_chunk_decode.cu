@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(DecodeShape<NB, MT>::kThreads, 1)
           }
         }
       };
-      if (tile0 + BN > sg.limit) {
+      if (sg.limit - tile0 < BN) {
         weigh(std::true_type{});
       } else {
         weigh(std::false_type{});

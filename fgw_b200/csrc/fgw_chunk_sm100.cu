@@ -158,7 +158,7 @@ __device__ __forceinline__ int tile_steps(const ChunkArgs& a, const ChunkSegment
   const int left = s.count - t * tokens;
   if (left <= 0) return 0;
   const int seen = seen_keys(a, s, t * tokens + min(left, tokens) - 1);
-  return max(0, min(s.n_begin + s.n, (seen + 127) / 128) - s.n_begin);
+  return max(0, min(s.n_begin + s.n, ceil_div<128>(seen)) - s.n_begin);
 }
 
 template <typename T, int NB>
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
         if (loads_v && wait_or_fail(&v_empty[st], parity, 82)) {
           // Rows past the last visible key, whatever the stage or the page holds there, must reach PV as zeros: the tile
           // that holds the end lands on a barrier of its own and becomes visible when they are zeroed.
-          const int past = (sg.n_begin + j) * BN + BN - sg.limit;
+          const int past = BN - (sg.limit - (sg.n_begin + j) * BN);
           uint64_t* landed = past > 0 ? v_raw : &v_full[st];
           if (lane == 0) mbar_arrive_expect_tx(landed, bytes);
           __syncwarp();

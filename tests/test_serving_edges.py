@@ -225,3 +225,28 @@ def test_attention_of_scores_that_are_not_finite(case, bad):
     assert np.array_equal(np.isnan(got), lost)
     bound = 2.0 ** -8 * (2 * np.abs(want) + spread) + 2.0 ** -16 * spread + 1e-6
     assert (np.abs(got - want)[~lost] <= bound[~lost]).all()
+
+
+# --- lengths near 2^31 ----------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 200], ids=["token", "chunk"])
+def test_attention_over_as_many_tokens_as_a_table_can_hold(new):
+    """2^31 - 16 cached tokens, over pages that repeat. The keys are zeros, so every weight is one and every sum a whole
+    number below 2^24 per CTA: the outputs are the values' shares, rounded once."""
+    from fgw_b200.operators.mha.chunk_attention import paged_chunk_attention
+    page, dim, pages = 16, 16, 8
+    width = 2 ** 27 - 1
+    table = (torch.arange(width, device="cuda", dtype=torch.int32) % pages).view(1, width)
+    lens = torch.tensor([width * page], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    k = torch.zeros(pages * page, 1, dim, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    v[:, :, 0] = 1  # every token
+    v[:page, :, 1] = 1  # every eighth page
+    v[3::page, :, 2] = 1  # one token of every page
+    v[5 * page + 7, :, 3] = 1
+    q = torch.randn(new, 1, dim, device="cuda").to(torch.bfloat16)
+    got = paged_chunk_attention(q, k, v, table, lens, cu, page).float()
+    for at, share in enumerate((1.0, 1 / 8, 1 / 16, 1 / 128)):
+        assert ((got[:, 0, at] - share).abs() <= share * 2.0 ** -8).all(), (at, got[:, 0, at])
+    assert not got[:, 0, 4:].any()
