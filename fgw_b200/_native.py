@@ -429,7 +429,8 @@ def torch_binding():
         spec.loader.exec_module(module)
     except ImportError as exc:
         raise NativeLibraryError(f"cannot load {path}: {exc}") from exc
-    if module.abi_version() != ABI_VERSION:
+    expected = (ABI_VERSION, *(ctypes.sizeof(kind) for kind in (ChunkParams, RotaryParams, PageParams)))
+    if getattr(module, "built_for", None) != expected:
         raise NativeLibraryError(f"{path} was built for another library: rebuild with `python -m fgw_b200.build`")
     _BINDING = module
     return module

@@ -56,20 +56,23 @@ def _compile(src, obj, extra):
     return proc.stderr
 
 
-def _build_binding():
-    """Compile the Python binding against the torch of this interpreter."""
+def binding_command(target, include=INCLUDE):
+    """The compiler call that makes the Python binding for the torch of this interpreter."""
     import torch
     from torch.utils import cpp_extension
 
-    includes = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], str(INCLUDE)]
+    includes = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], str(include)]
     libraries = cpp_extension.library_paths("cuda")
+    return ["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=fgw_torch",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[flag for path in includes for flag in ("-isystem", path)], str(BINDING_SOURCE), "-o", str(target),
+            f"-L{LIB_DIR}", *[f"-L{path}" for path in libraries], "-lfgw_mha", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+
+
+def _build_binding():
     tmp = BINDING.with_suffix(".so.tmp")
-    cmd = ["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=fgw_torch",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[flag for path in includes for flag in ("-isystem", path)], str(BINDING_SOURCE), "-o", str(tmp),
-           f"-L{LIB_DIR}", *[f"-L{path}" for path in libraries], "-lfgw_mha", "-lc10", "-lc10_cuda", "-ltorch_cpu",
-           "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+    proc = subprocess.run(binding_command(tmp), capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDING_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, BINDING)

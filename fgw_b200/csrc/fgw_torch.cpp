@@ -306,7 +306,9 @@ void copy_pages(const std::vector<at::Tensor>& pools, const at::Tensor& src, con
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("abi_version", &fgw_mha_abi_version);
+  // the header this file was compiled with: its version, and the sizes of the structures it passes
+  m.attr("built_for") = pybind11::make_tuple(FGW_MHA_ABI_VERSION, sizeof(fgw_chunk_params), sizeof(fgw_rotary_params),
+                                             sizeof(fgw_page_params));
   m.def("paged_chunk_attention", &paged_chunk_attention);
   m.def("rotary_append", &rotary_append);
   m.def("fork_pages", &fork_pages);

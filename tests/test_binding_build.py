@@ -1,0 +1,27 @@
+"""The compiled binding of the serving-step operators: what it was built for, and when it is built."""
+import subprocess
+import sys
+
+from fgw_b200 import _native, build
+
+
+def test_a_binding_of_another_header_is_refused(tmp_path):
+    """A binding left over from an older header would hand over structures of another layout."""
+    header = (build.INCLUDE / "fgw_mha.h").read_text()
+    line = f"#define FGW_MHA_ABI_VERSION {_native.ABI_VERSION}\n"
+    assert line in header
+    include, lib = tmp_path / "include", tmp_path / "lib"
+    include.mkdir()
+    lib.mkdir()
+    (include / "fgw_mha.h").write_text(header.replace(line, "#define FGW_MHA_ABI_VERSION 4\n"))
+    (lib / build.LIB.name).symlink_to(build.LIB)
+    made = subprocess.run([*build.binding_command(lib / build.BINDING.name, include), "-O0"], capture_output=True, text=True)
+    assert made.returncode == 0, made.stderr
+    # in a process of its own: a process has one module of the name
+    load = ("import pathlib, sys; from fgw_b200 import _native; _native.LIB_PATH = pathlib.Path(sys.argv[1])\n"
+            "try: _native.torch_binding()\n"
+            "except _native.NativeLibraryError as error: print('refused:', error)")
+    ran = subprocess.run([sys.executable, "-c", load, str(lib / build.LIB.name)], capture_output=True, text=True,
+                         cwd=build.ROOT)
+    assert ran.returncode == 0 and ran.stdout.startswith("refused:") and "rebuild" in ran.stdout, ran
+    _native.torch_binding()  # the tree's own is good
