@@ -10,6 +10,8 @@ sources and headers are kept).
 """
 import argparse
 import concurrent.futures
+import importlib.metadata
+import importlib.util
 import os
 import pathlib
 import shutil
@@ -26,6 +28,7 @@ LIB_DIR = PACKAGE / "_lib"
 LIB = LIB_DIR / "libfgw_mha.so"
 BINDING = LIB_DIR / "fgw_torch.so"
 BINDING_SOURCE = CSRC / "fgw_torch.cpp"
+BINDING_STAMP = BUILD / "fgw_torch.built_for"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # Host code keeps separate multiplies and adds (no fused multiply-add contraction): the host split choice
@@ -54,6 +57,12 @@ def _compile(src, obj, extra):
     if proc.returncode != 0:
         raise RuntimeError(f"nvcc failed for {src.name}:\n{proc.stdout}\n{proc.stderr}")
     return proc.stderr
+
+
+def _version(package):
+    """Version and place of an installed package, without importing it; None if there is none."""
+    spec = importlib.util.find_spec(package)
+    return None if spec is None else f"{importlib.metadata.version(package)} {spec.origin}"
 
 
 def binding_command(target, include=INCLUDE):
@@ -101,8 +110,12 @@ def build(force=False, jobs=None, verbose_ptxas=False):
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
         os.replace(tmp, LIB)
-    if force or _stale(BINDING, BINDING_SOURCE, sorted(INCLUDE.glob("*.h"))):
+    # the binding is compiled against the interpreter's and torch's headers, which are not among its sources
+    built_for = f"torch {_version('torch')}\npython {sys.version}\n"
+    if (force or _stale(BINDING, BINDING_SOURCE, sorted(INCLUDE.glob("*.h")))
+            or not BINDING_STAMP.exists() or BINDING_STAMP.read_text() != built_for):
         _build_binding()
+        BINDING_STAMP.write_text(built_for)
     if verbose_ptxas:
         for name, text in sorted(logs.items()):
             print(f"== {name}\n{text}")

@@ -25,3 +25,27 @@ def test_a_binding_of_another_header_is_refused(tmp_path):
                          cwd=build.ROOT)
     assert ran.returncode == 0 and ran.stdout.startswith("refused:") and "rebuild" in ran.stdout, ran
     _native.torch_binding()  # the tree's own is good
+
+
+def binding_builds(monkeypatch):
+    """How often build() makes the binding from here on (the compiler is not run)."""
+    made = []
+    monkeypatch.setattr(build, "_build_binding", lambda: made.append(1))
+    return made
+
+
+def test_the_binding_is_built_again_for_another_torch_or_python(tmp_path, monkeypatch):
+    made = binding_builds(monkeypatch)
+    monkeypatch.setattr(build, "BINDING_STAMP", tmp_path / "stamp")
+    build.build()
+    assert len(made) == 1  # nothing says what the present one was built with
+    build.build()
+    assert len(made) == 1
+    monkeypatch.setattr(build, "_version", lambda package: "0.0+other")
+    build.build()
+    assert len(made) == 2
+    build.build()
+    assert len(made) == 2
+    monkeypatch.setattr(build.sys, "version", "another interpreter")
+    build.build()
+    assert len(made) == 3
