@@ -3,7 +3,7 @@
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` in parallel; the objects link into
 ``fgw_b200/_lib/libfgw_mha.so`` with the CUDA runtime linked statically, so the library only
 needs the NVIDIA driver at run time. ``csrc/fgw_torch.cpp`` becomes ``fgw_b200/_lib/fgw_torch.so`` beside it (a
-Python extension on torch's headers that calls the library). Re-running is incremental (objects newer than their
+Python extension on torch's headers that calls the library; left out where torch is not installed). Re-running is incremental (objects newer than their
 sources and headers are kept).
 
     python -m fgw_b200.build [--force] [--jobs N]
@@ -112,8 +112,10 @@ def build(force=False, jobs=None, verbose_ptxas=False):
         os.replace(tmp, LIB)
     # the binding is compiled against the interpreter's and torch's headers, which are not among its sources
     built_for = f"torch {_version('torch')}\npython {sys.version}\n"
-    if (force or _stale(BINDING, BINDING_SOURCE, sorted(INCLUDE.glob("*.h")))
-            or not BINDING_STAMP.exists() or BINDING_STAMP.read_text() != built_for):
+    if _version("torch") is None:
+        print("the binding of the serving-step operators is left out: built without torch")
+    elif (force or _stale(BINDING, BINDING_SOURCE, sorted(INCLUDE.glob("*.h")))
+          or not BINDING_STAMP.exists() or BINDING_STAMP.read_text() != built_for):
         _build_binding()
         BINDING_STAMP.write_text(built_for)
     if verbose_ptxas:

@@ -49,3 +49,14 @@ def test_the_binding_is_built_again_for_another_torch_or_python(tmp_path, monkey
     monkeypatch.setattr(build.sys, "version", "another interpreter")
     build.build()
     assert len(made) == 3
+
+
+def test_the_library_builds_without_torch(tmp_path):
+    """Users of the C ABI need no torch: the library is built, the binding left out."""
+    run = ("import pathlib, sys; sys.modules['torch'] = None; from fgw_b200 import build\n"
+           "build.BINDING = pathlib.Path(sys.argv[1]); build.BINDING_STAMP = build.BINDING.with_suffix('.stamp')\n"
+           "print(build.build() == build.LIB, build.BINDING.exists())")
+    ran = subprocess.run([sys.executable, "-c", run, str(tmp_path / "fgw_torch.so")], capture_output=True, text=True,
+                         cwd=build.ROOT)
+    assert ran.returncode == 0, ran.stderr
+    assert ran.stdout.splitlines()[-1] == "True False" and "without torch" in ran.stdout
