@@ -103,7 +103,8 @@ def compact_pages(table, lens, page, pages):
     held = [-(-min(max(int(n), 0), width * page) // page) for n in lens]
     used = sorted({int(e) for b in range(rows) for e in table[b, :held[b]] if 0 <= e < pages})
     live = len(used)
-    holes = [e for e in range(live) if e not in set(used)]
+    kept = set(used)
+    holes = [e for e in range(live) if e not in kept]
     to = dict(zip([e for e in used if e >= live], holes))
     out = np.full_like(table, -1)
     for b in range(rows):

@@ -11,7 +11,7 @@ import torch
 
 from fgw_b200 import _native
 from oracle import serving
-from test_serving_ops import attend_case, on_gpu, values
+from test_serving_ops import attend_case, on_gpu, ragged, torch_attention, values
 
 MAX_ENTRIES = 2 ** 31 - 2 ** 16
 
@@ -250,3 +250,87 @@ def test_attention_over_as_many_tokens_as_a_table_can_hold(new):
     for at, share in enumerate((1.0, 1 / 8, 1 / 16, 1 / 128)):
         assert ((got[:, 0, at] - share).abs() <= share * 2.0 ** -8).all(), (at, got[:, 0, at])
     assert not got[:, 0, 4:].any()
+
+
+# --- sizes at which the kernels take their other paths ----------------------------------------------------------------
+BIG_STATES = [
+    # (name, held, page, spare pages): more than 4096 rows, 32768 table entries, 131072 pages; the last has just as many
+    ("rows", [(7 * i) % 33 for i in range(5000)], 4, 30000),
+    ("entries", [37 * i % 1200 for i in range(1, 65)], 2, 3000),
+    ("pages", [100 * i for i in range(9)], 4, 140000),
+    ("below", [5 * i % 28 for i in range(4096)], 4, 131072 - 15354),
+]
+
+
+def big_state(case, row=(8,)):
+    name, held, page, spare = case
+    table, lens, _, pages = ragged([0] * len(held), held, page, 7, spare_pages=spare, spare_width=1)
+    return table, lens, pages, page, values((pages * page, *row), torch.float16, 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", BIG_STATES, ids=[c[0] for c in BIG_STATES])
+def test_fork_of_large_tables(case):
+    from fgw_b200.operators.mha.page_ops import fork_pages
+    table, lens, pages, page, store = big_state(case)
+    rng = np.random.default_rng(3)
+    rows = len(lens)
+    parents = np.where(rng.random(rows) < 0.5, np.arange(rows), rng.integers(-1, rows, rows)).astype(np.int32)
+    lens[1::7] -= np.minimum(lens[1::7], 1)  # ends that are not where the tables were filled to
+    table[2::11] = table[1::11][:len(table[2::11])]  # rows that hold their neighbours' pages, also with other lengths
+    lens[2::11] = np.minimum(lens[2::11], lens[1::11][:len(lens[2::11])])
+    held = np.where(parents >= 0, lens[np.maximum(parents, 0)], 0)
+    reserve = (held + rng.integers(0, 3, rows)).astype(np.int32)
+    want_table, want_lens, want_status, copies = serving.fork_pages(table, lens, parents, reserve, page, pages)
+    assert want_status[0] <= want_status[1] and len(copies) >= 2
+    pool = store.cuda()
+    got = fork_pages([pool], *on_gpu(table, lens, parents), page, reserve_seqlens=on_gpu(reserve)[0])
+    assert tuple(got[2].tolist()) == want_status
+    assert np.array_equal(got[0].cpu().numpy(), want_table) and np.array_equal(got[1].cpu().numpy(), want_lens)
+    assert torch.equal(pool.cpu().view(torch.int16),
+                       torch.from_numpy(serving.copy_rows(store.view(torch.int16).numpy(), copies, page)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", BIG_STATES, ids=[c[0] for c in BIG_STATES])
+def test_compaction_of_large_tables(case):
+    from fgw_b200.operators.mha.page_ops import compact_pages
+    table, lens, pages, page, store = big_state(case)
+    table[2::11] = table[1::11][:len(table[2::11])]
+    lens[2::11] = np.minimum(lens[2::11], lens[1::11][:len(lens[2::11])])
+    want_table, want_status, copies = serving.compact_pages(table, lens, page, pages)
+    pool = store.cuda()
+    got, status = compact_pages([pool], *on_gpu(table, lens), page)
+    assert tuple(status.tolist()) == want_status and want_status[1] > 50
+    assert np.array_equal(got.cpu().numpy(), want_table)
+    assert torch.equal(pool.cpu().view(torch.int16),
+                       torch.from_numpy(serving.copy_rows(store.view(torch.int16).numpy(), copies, page)))
+
+
+MANY_REQUESTS = [
+    # (name, new, held, heads, kv heads, dim, page, causal): more requests than threads share out one each (288), than the
+    # plan sorts (2048), and more items than it sorts
+    ("tokens_300", [1] * 300, [(13 * i) % 200 for i in range(300)], 4, 2, 64, 16, True),
+    ("tokens_2100", [int(i % 5 > 0) for i in range(2100)], [1 + (29 * i) % 90 for i in range(2100)], 2, 1, 32, 16, True),
+    ("mixed_600", [(0, 1, 1, 40, 3, 1, 200)[i % 7] for i in range(600)], [200 + (17 * i) % 150 for i in range(600)], 2, 1,
+     64, 16, True),
+    ("mixed_2100", [(0, 1, 1, 2, 300)[i % 5] if i % 50 < 5 else 1 for i in range(2100)],
+     [300 + (11 * i) % 60 for i in range(2100)], 2, 2, 32, 16, True),
+    ("chunks_2100", [33 + i % 3 for i in range(2100)], [40 + (7 * i) % 200 for i in range(2100)], 2, 1, 16, 16, True),
+    ("items_of_one_token", [900, 1, 700, 650], [1000, 40, 700, 900], 128, 1, 256, 64, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MANY_REQUESTS, ids=[c[0] for c in MANY_REQUESTS])
+def test_attention_of_many_requests(case):
+    from fgw_b200.operators.mha.chunk_attention import paged_chunk_attention
+    _, new, held, heads, kv_heads, dim, page, causal = case
+    q, k, v, table, lens, cu = attend_case(case, torch.bfloat16, seed=51)
+    args = [q.cuda(), k.cuda(), v.cuda()]
+    out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
+    got = paged_chunk_attention(*args, *on_gpu(table, lens, cu), page, is_causal=causal, out=out)
+    want, spread = torch_attention(*args, table, lens, cu, page, causal)
+    bound = 2.0 ** -8 * (2 * want.abs() + spread) + 2.0 ** -16 * spread + 1e-6
+    assert bool(((got.double() - want).abs() <= bound).all())
+    assert torch.equal(got, paged_chunk_attention(*args, *on_gpu(table, lens, cu), page, is_causal=causal))
