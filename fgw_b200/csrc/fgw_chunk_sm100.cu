@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
     }
     bool ok = true;
     uint32_t kc = 0, qc = 0, raw = 0;
-    uint32_t issued = 0, issued_q = 0;  // K or V tiles and query tiles loaded, whose barriers complete when they land
+    uint32_t given_up = 0, given_up_q = 0;  // kc and qc when a wait gave up: nothing is loaded from there on
     const int boxes = BN / a.box_rows;
     const int box = lane % boxes, blk = lane / boxes;
     const uint32_t box_bytes = a.box_rows * 128;
@@ -248,6 +248,8 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
     auto wait_or_fail = [&](uint64_t* bar, uint32_t parity, int site) {
       if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity, a.budget_ns))) {
         ok = false;
+        given_up = kc;
+        given_up_q = qc;
         if (lane == 0) chunk_error(a, site);
       }
       return ok;
@@ -261,7 +263,6 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
       if (loads_k && wait_or_fail(q_empty, (qc & 1) ^ 1, 80) && lane == 0) {
         const int tiles_q = kTiles == 2 && sg.count > tile_tokens ? 2 : 1;
         mbar_arrive_expect_tx(q_full, tiles_q * NB * q_bytes);
-        ++issued_q;
         for (int t = 0; t < tiles_q; ++t) {
           for (int b = 0; b < NB; ++b) {
             tma_load_4d(q_smem + t * S::kQBytes + b * S::kTileBytes, &qmap, q_full, b * 64, 0, sg.hk,
@@ -284,7 +285,6 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
           if (lane == 0) mbar_arrive_expect_tx(&k_full[st], bytes);
           __syncwarp();
           if (load) tma_load_3d(dst, &kmap, &k_full[st], blk * 64, sg.hk, row);
-          ++issued;
         }
         if (loads_v && wait_or_fail(&v_empty[st], parity, 82)) {
           // Rows past the last visible key, whatever the stage or the page holds there, must reach PV as zeros: the tile
@@ -294,13 +294,7 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
           if (lane == 0) mbar_arrive_expect_tx(landed, bytes);
           __syncwarp();
           if (load) tma_load_3d(dst + (S::kV - S::kK), &vmap, landed, blk * 64, sg.hk, row);
-          if (past <= 0) {
-            ++issued;
-          } else if (!wait_or_fail(v_raw, raw & 1, 92)) {
-            mbar_wait(v_raw, raw & 1, kDrainBudgetNs);  // the copy in flight; v_full is not going to complete
-          } else {
-            ++raw;
-            ++issued;
+          if (past > 0 && wait_or_fail(v_raw, raw++ & 1, 92)) {
             uint8_t* end = v_smem + st * S::kKVBytes + (BN - past) * 128;  // whole 128-byte rows: swizzled within
             for (int i = lane; i < past * 8; i += 32) {
 #pragma unroll
@@ -314,13 +308,15 @@ __global__ void __launch_bounds__(TensorShape<NB>::kThreads, 1)
         ++kc;
       }
     }
-    // Leave no copy in flight, whichever role gave up: the last load of every stage lands before the CTA may end. Nothing
-    // is issued after a wait gave up, so the i-th load went to stage i % NS.
+    // Leave no copy in flight, whichever role gave up: the last load of every stage lands before the CTA may end.
+    const uint32_t loaded = ok ? kc : given_up, loaded_q = ok ? qc : given_up_q;
     uint64_t* full = loads_k ? k_full : v_full;
-    for (uint32_t i = issued > NS ? issued - NS : 0; i < issued; ++i) {
+    for (uint32_t i = loaded > NS ? loaded - NS : 0; i < loaded; ++i) {
       mbar_wait(&full[i % NS], (i / NS) & 1, kDrainBudgetNs);
     }
-    if (issued_q > 0) mbar_wait(q_full, (issued_q - 1) & 1, kDrainBudgetNs);
+    if (loads_k && loaded_q > 0) mbar_wait(q_full, (loaded_q - 1) & 1, kDrainBudgetNs);
+    // a ragged V tile lands on a barrier of its own, also the one whose wait gave up
+    if (loads_v && raw > 0) mbar_wait(v_raw, (raw - 1) & 1, kDrainBudgetNs);
   } else if (warp <= kTiles) {
     // ------------------------------------------------------------------------- MMA issuer
     // One warp per query tile, so that one tile's waits do not hold up the other's MMAs; a K or V stage, and Q, are free
