@@ -259,15 +259,15 @@ __device__ __forceinline__ void page_plan(PageArgs a, int* shared) {
   };
   if (kFork) {
     for (int i = tid; i < a.batch; i += kThreads) {
-      const ForkRow r = fork_row(a, i);
+      const int parent = fresh(&a.ws.rows[i].x), full = fresh(&a.ws.rows[i].y), held = fresh(&a.ws.rows[i].w);
       bool copies = false;
-      if (r.held > r.full) {
-        const int end = a.table[static_cast<long long>(r.parent) * a.width + r.full];
-        copies = fresh(&a.ws.first[r.parent]) != i ||
+      if (held > full) {
+        const int end = a.table[static_cast<long long>(parent) * a.width + full];
+        copies = fresh(&a.ws.first[parent]) != i ||
                  (end >= 0 && end < a.pages && (fresh(&a.ws.shut[end >> 5]) >> (end & 31) & 1) != 0);
       }
-      a.ws.need[i] = (copies ? 1 : 0) + r.want - r.held;
-      if (!copies) a.ws.rows[i].y = r.held;
+      a.ws.need[i] = (copies ? 1 : 0) + fresh(&a.ws.rows[i].z) - held;
+      if (!copies) a.ws.rows[i].y = held;
     }
   }
   for (int b = warp; b < a.blocks; b += kWarps) {
