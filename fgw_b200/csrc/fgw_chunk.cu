@@ -61,7 +61,8 @@ __device__ __forceinline__ V block_scan(V v, V& total, V* shared) {
 // by more than 5 % and what cutting costs, only as many rounds are whole as stay within each program's share, and the rest
 // is cut into a contiguous range of units per program that fills its share up. The last round by load, against snake
 // order throughout: a batch of prompts 64.6 -> 58.3 us (CTAs of 28 to 53 us -> 28 to 45), single tokens and chunks
-// mixed 160.9 -> 158.4 us.
+// mixed 160.9 -> 158.4 us. The sort compares every row with every other: nothing for the tens of rows of such a step, but
+// 193 us for 2000 requests of 70 tokens, whose items then take 262.
 struct PlanShared {
   long long scan_l[32];
   int scan_i[32];
@@ -418,6 +419,9 @@ CUresult chunk_kv_maps(CUtensorMap* kmap, CUtensorMap* vmap, const fgw_chunk_par
 // among them) for single tokens, which are then its work. 33 to 64 rows, against the tensor kernel: D = 256, 13 requests of
 // 56 rows over 2000 keys 54.2 -> 34.7 us, 8 of 40 over 8000 with two key heads 80.2 -> 67.8 us, 32 of 64 over 3000 65.1 ->
 // 62.2 us; D = 192, 32 of 64 over 3000 49.8 -> 53.1 us, where many requests fill the tensor kernel too.
+// Going by the average is its weak spot: where it is at most 64, a long chunk among many single tokens goes through this
+// kernel too, in items of so few rows that its cache is read again for each (32 heads on 8 of 128, 199 tokens over caches to
+// 8K: 615 us; with a chunk of 64 637, of 512 798, of 2048 2631, of 3500, which the average gives away, 854 us).
 static int decode_rows(const fgw_chunk_params& p) {
   constexpr long long most = 64;
   const long long group = p.heads / p.kv_heads;

@@ -15,7 +15,7 @@
 // range. That costs two or three trips to L2 before the first load; a plan kernel ahead of it took 6 us by itself. Divisions by
 // variables, chains of which stood between those trips, are multiplications (FastDiv): 18.3 to 14.2 us.
 //
-// Measured: 64 tokens over caches of up to 8K (1.28 GB, pages of 16) 214 us, 5.96 TB/s, 0.91 of the copy rate; the rest is
+// Measured: 64 tokens over caches of up to 8K (1.28 GB, pages of 16) 216 us, 5.91 TB/s, 0.90 of the copy rate; the rest is
 // the start (cursor, first loads) and the merge, some 14 us in all. Eight tokens over 1K (21 MB): 14 us, of which
 // the start takes 3, the stream 4 and the merge kernel 4.
 #include <algorithm>

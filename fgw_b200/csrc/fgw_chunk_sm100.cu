@@ -13,7 +13,7 @@
 // Bound by the softmax's chain of waits, TMEM loads, maximum, 2^x and TMEM stores, far more than by any unit: a tile pair
 // costs 2048 cycles of 2^x whatever D is and 1024 (D = 64) or 2048 (D = 128) of MMA, and a step takes 3600 to 4000. At
 // D = 64 a step without its MMAs takes as long, without its 2^x 0.8 of the time. Measured: 4096 tokens over 28K cached, 32
-// heads on 8 key heads of 128, 1790 us = 1.15 PFLOP/s; 16 requests of chunks and single tokens, 24 heads on 8 of 64, 154 us;
+// heads on 8 key heads of 128, 1790 to 1914 us by the card's clock = 1.08 to 1.15 PFLOP/s; 16 requests of chunks and single tokens, 24 heads on 8 of 64, 154 us;
 // 8 prompts of up to 1024, 16 heads of 128, 53.5 us. At D = 64, steps kept and what they replaced: P apart, two warpgroups
 // per tile, an MMA warp per tile, turns together 165 -> 159 us. Tried and slower or without effect: two warpgroups per
 // tile at D = 128 (1902 to 2478 us, by the spills), a third score buffer (178 to 192 us), QK of the next item issued beside

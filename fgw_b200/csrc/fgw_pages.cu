@@ -12,7 +12,8 @@
 // up to 128K pages are one CTA's work with the bitmap and the row arrays in shared memory; larger ones go to a cluster
 // of eight CTAs over global memory (eight rows over one layer: 9.7 against 11.8 us with the copy). page_copy_kernel then
 // moves the bytes, bound by HBM; it is launched beside the plan and waits for it. Measured: 700 pages of 128 KB in 8 pools
-// (1.47 GB read and written) 258 us, 5.7 TB/s; 55 half-filled pages in 16 pools 28 us, of which the plan takes 10.
+// (1.47 GB read and written) 257 us, 5.7 TB/s; 55 half-filled pages in 16 pools 28 us, of which the plan takes 10. That
+// ends which other rows hold are told from ends that only forks of one row share is a second bitmap: no time that shows.
 #include <cooperative_groups.h>
 
 #include <algorithm>

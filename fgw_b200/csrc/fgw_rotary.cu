@@ -10,7 +10,9 @@
 // the offsets, so a large batch costs two or three loads in a row, not log2(batch). What kept it from the memory's rate
 // was loads in flight: the first form, two heads at a time after the places were known, took 51.0 us for 219 MB; three
 // heads, loaded while the places are found or the batch before is turned, 43.4 us; CTAs of 128 threads instead of 256,
-// so that more of them are at different points, 40.6 us (5.4 TB/s).
+// so that more of them are at different points, 40.8 us (5.4 TB/s). Rotary parts whose halves are no whole 16-byte chunks
+// go value by value, which the instructions bound: 8192 tokens, 32 heads on 8 of 96, 24 rotated in halves 188 us, where
+// adjacent pairs, which keep the chunks, take 31.6.
 #include <algorithm>
 
 #include "fgw_common.cuh"

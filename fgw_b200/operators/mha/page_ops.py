@@ -3,7 +3,8 @@
 The table and the lengths alone say which pages are live: row b holds the pages of its first ``cache_seqlens[b]`` tokens,
 and a page that no row holds is free. So there is no free list or count to keep in step; whoever keeps pages outside
 the batch (a prefix cache) keeps them as rows of the table. Everything stays on the device: the calls read no length
-on the host, and give new tables, so that a step in flight can go on reading the old ones.
+on the host, and give new tables, so that a step launched before on the same stream reads the old ones. A step on another
+stream has to be waited for: pages that a fork frees may be given out and written by the same call.
 
 ``pools`` are the K and V caches of every layer, a list of tensors of one shape [num_pages * page_size, ...] and type
 whose rows are multiples of 16 bytes. Arguments that do not fit raise ValueError before any launch.

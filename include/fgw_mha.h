@@ -293,7 +293,8 @@ FGW_API int fgw_paged_cache_gather(const fgw_gather_params* params, void* stream
  * Ragged batches: request b's new tokens are rows cu_seqlens_q[b] <= t < cu_seqlens_q[b + 1] of q, k, v and out, in
  * order; cache_seqlens[b] counts its tokens in the cache WITH the new ones, so the i-th of n new tokens has position
  * cache_seqlens[b] - n + i. All lengths stay device data: no call copies to the host or synchronises. cu_seqlens_q is
- * non-decreasing; lengths are clamped into [0, table_width * page_size].
+ * non-decreasing. Lengths belong into [0, table_width * page_size]: attention and the page operators clamp them, the
+ * rotary append drops the positions that are past it.
  */
 
 /*
